@@ -353,6 +353,80 @@ FlashAttentionError cp_bwd_finish_impl(const void* ws, T* dQ, int nq, int B, int
     return cuflash::detail::launch_bwd_cp_finish_sm100<T>(ws, dQ, nq, B * H, C, D, scale, stream);
 }
 
+// Page geometry shared by the paged-cache entries: page_size a power of two,
+// the tables' token range and the pool's rows within 32 bits.
+bool paged_geometry_ok(int page_size, int max_pages, int num_pages) {
+    return page_size > 0 && (page_size & (page_size - 1)) == 0 && max_pages > 0 &&
+           num_pages > 0 && static_cast<long long>(max_pages) * page_size <= 0x7fffffffLL &&
+           static_cast<long long>(num_pages) * page_size <= 0x7fffffffLL;
+}
+
+template <typename T>
+FlashAttentionError kv_append_impl(const T* Q, const T* K, const T* V, T* Q_out, T* K_cache,
+                                   T* V_cache, const float* rope, const int* positions,
+                                   const int* block_table, const int* seq_lens,
+                                   const int* cu_seqlens, int num_tokens, int B, int Hq, int Hkv,
+                                   int D, int page_size, int max_pages, int num_pages,
+                                   long long q_stride, long long k_stride, long long v_stride,
+                                   int rotary_dim, int max_position, bool interleaved,
+                                   cudaStream_t stream) {
+    if (!K || !V || !K_cache || !V_cache || !block_table || !seq_lens || !Q != !Q_out)
+        return FlashAttentionError::NULL_POINTER;
+    if (num_tokens <= 0 || B <= 0 || Hkv <= 0 || D <= 0 || (Q && Hq <= 0))
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (!paged_geometry_ok(page_size, max_pages, num_pages))
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (!cu_seqlens && num_tokens != B) return FlashAttentionError::DIMENSION_MISMATCH;
+    if (!(D == 32 || D == 64 || D == 128)) return FlashAttentionError::UNSUPPORTED_HEAD_DIM;
+    if (rope && (rotary_dim <= 0 || rotary_dim % 16 != 0 || rotary_dim > D || max_position <= 0))
+        return FlashAttentionError::INVALID_DIMENSION;
+    // a token's heads are contiguous and its rows 16-byte aligned
+    const long long need[3] = {Q ? static_cast<long long>(Hq) * D : 0,
+                               static_cast<long long>(Hkv) * D, static_cast<long long>(Hkv) * D};
+    const long long stride[3] = {q_stride, k_stride, v_stride};
+    for (int i = 0; i < 3; ++i)
+        if (stride[i] != 0 && (stride[i] < need[i] || stride[i] % 8 != 0))
+            return FlashAttentionError::INVALID_DIMENSION;
+    // in place only where every head is read before its own place is written
+    if (Q && static_cast<const void*>(Q) == static_cast<void*>(Q_out) && q_stride != 0 &&
+        q_stride != need[0])
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (cuflash::detail::sticky_failure()) return FlashAttentionError::CUDA_ERROR;
+    return cuflash::detail::launch_kv_append<T>(
+        Q, K, V, Q_out, K_cache, V_cache, rope, positions, block_table, seq_lens, cu_seqlens,
+        num_tokens, B, Hq, Hkv, D, page_size, max_pages, num_pages, q_stride, k_stride, v_stride,
+        rotary_dim, max_position, interleaved, stream);
+}
+
+// Ragged attention (paged == true) or shared-prefix decode over a paged cache.
+template <typename T>
+FlashAttentionError paged_attention_impl(bool shared_prefix, const T* Q, const T* K, const T* V,
+                                         const int* prefix_table, const int* prefix_len,
+                                         const int* block_table, const int* seq_lens,
+                                         const int* cu_seqlens, T* O, float* L, int num_tokens,
+                                         int B, int Hq, int Hkv, int D, int page_size,
+                                         int max_prefix_pages, int max_pages, int num_pages,
+                                         float scale, bool causal, cudaStream_t stream) {
+    if (!Q || !K || !V || !O || !L || !block_table || !seq_lens)
+        return FlashAttentionError::NULL_POINTER;
+    if (shared_prefix ? (!prefix_table || !prefix_len) : !cu_seqlens)
+        return FlashAttentionError::NULL_POINTER;
+    if (num_tokens <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0)
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (!paged_geometry_ok(page_size, max_pages, num_pages) ||
+        (shared_prefix && !paged_geometry_ok(page_size, max_prefix_pages, num_pages)))
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (Hq % Hkv != 0) return FlashAttentionError::DIMENSION_MISMATCH;
+    if (!(D == 32 || D == 64 || D == 128)) return FlashAttentionError::UNSUPPORTED_HEAD_DIM;
+    if (!std::isfinite(scale) || scale < 0.0f) return FlashAttentionError::INVALID_DIMENSION;
+    if (static_cast<long long>(num_tokens) * Hq > 0x7fffffffLL)
+        return FlashAttentionError::INVALID_DIMENSION;
+    if (cuflash::detail::sticky_failure()) return FlashAttentionError::CUDA_ERROR;
+    return cuflash::detail::launch_paged_attention<T>(
+        Q, K, V, prefix_table, prefix_len, block_table, seq_lens, cu_seqlens, O, L, num_tokens, B,
+        Hq, Hkv, D, page_size, max_prefix_pages, max_pages, num_pages, scale, causal, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -659,6 +733,45 @@ int cuflash_attention_decode_bf16_noalloc(const __nv_bfloat16* Q, const __nv_bfl
     return static_cast<int>(cuflash::detail::launch_decode_bf16_noalloc(
         Q, K, V, O, L, batch_size, num_heads, kv_len, head_dim, scale, num_splits, stream));
 }
+
+#define CUFLASH_PAGED_ENTRIES(SUFFIX, T)                                                           \
+    int cuflash_kv_append_paged_##SUFFIX(                                                          \
+        const T* Q, const T* K, const T* V, T* Q_out, T* K_cache, T* V_cache,                      \
+        const float* rope_table, const int* positions, const int* block_table,                     \
+        const int* seq_lens, const int* cu_seqlens, int num_tokens, int batch_size,                \
+        int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages_per_seq,     \
+        int num_pages, long long q_stride, long long k_stride, long long v_stride, int rotary_dim, \
+        int max_position, bool interleaved, cudaStream_t stream) {                                 \
+        return static_cast<int>(kv_append_impl<T>(                                                 \
+            Q, K, V, Q_out, K_cache, V_cache, rope_table, positions, block_table, seq_lens,        \
+            cu_seqlens, num_tokens, batch_size, num_q_heads, num_kv_heads, head_dim, page_size,    \
+            max_pages_per_seq, num_pages, q_stride, k_stride, v_stride, rotary_dim, max_position,  \
+            interleaved, stream));                                                                 \
+    }                                                                                              \
+    int cuflash_attention_forward_paged_##SUFFIX(                                                  \
+        const T* Q, const T* K_cache, const T* V_cache, const int* block_table,                    \
+        const int* seq_lens, const int* cu_seqlens, T* O, float* L, int num_tokens,                \
+        int batch_size, int num_q_heads, int num_kv_heads, int head_dim, int page_size,            \
+        int max_pages_per_seq, int num_pages, float scale, bool causal, cudaStream_t stream) {     \
+        return static_cast<int>(paged_attention_impl<T>(                                           \
+            false, Q, K_cache, V_cache, nullptr, nullptr, block_table, seq_lens, cu_seqlens, O, L, \
+            num_tokens, batch_size, num_q_heads, num_kv_heads, head_dim, page_size, 0,             \
+            max_pages_per_seq, num_pages, scale, causal, stream));                                 \
+    }                                                                                              \
+    int cuflash_attention_decode_shared_prefix_##SUFFIX(                                           \
+        const T* Q, const T* K_cache, const T* V_cache, const int* prefix_table,                   \
+        const int* prefix_len, const int* block_table, const int* seq_lens, T* O, float* L,        \
+        int batch_size, int num_q_heads, int num_kv_heads, int head_dim, int page_size,            \
+        int max_prefix_pages, int max_pages_per_seq, int num_pages, float scale,                   \
+        cudaStream_t stream) {                                                                     \
+        return static_cast<int>(paged_attention_impl<T>(                                           \
+            true, Q, K_cache, V_cache, prefix_table, prefix_len, block_table, seq_lens, nullptr,   \
+            O, L, batch_size, batch_size, num_q_heads, num_kv_heads, head_dim, page_size,          \
+            max_prefix_pages, max_pages_per_seq, num_pages, scale, false, stream));                \
+    }
+CUFLASH_PAGED_ENTRIES(bf16, __nv_bfloat16)
+CUFLASH_PAGED_ENTRIES(f16, half)
+#undef CUFLASH_PAGED_ENTRIES
 
 int cuflash_device_status(void) { return cuflash::detail::read_and_clear_device_status(); }
 

@@ -194,6 +194,31 @@ FlashAttentionError launch_decode_bf16_noalloc(const __nv_bfloat16* Q, const __n
                                                int B, int H, int kv_len, int D, float scale,
                                                int num_splits, cudaStream_t stream);
 
+// Keys and values into a paged cache, rotated on the way (kv_append.cu).
+// Q / Q_out nullptr: none; rope nullptr: no rotation; cu_seqlens nullptr: one
+// token per sequence; strides in elements between tokens, 0: contiguous.
+template <typename T>
+FlashAttentionError launch_kv_append(const T* Q, const T* K, const T* V, T* Q_out, T* K_cache,
+                                     T* V_cache, const float* rope, const int* positions,
+                                     const int* block_table, const int* seq_lens,
+                                     const int* cu_seqlens, int num_tokens, int B, int Hq, int Hkv,
+                                     int D, int page_size, int max_pages, int num_pages,
+                                     long long q_stride, long long k_stride, long long v_stride,
+                                     int rotary_dim, int max_position, bool interleaved,
+                                     cudaStream_t stream);
+
+// Attention over a paged cache (paged_sm100.cu): ragged tokens per sequence
+// (prefix_table nullptr) or one token per sequence behind a shared prefix
+// (cu_seqlens nullptr).
+template <typename T>
+FlashAttentionError launch_paged_attention(const T* Q, const T* K_cache, const T* V_cache,
+                                           const int* prefix_table, const int* prefix_len,
+                                           const int* block_table, const int* seq_lens,
+                                           const int* cu_seqlens, T* O, float* L, int num_tokens,
+                                           int B, int Hq, int Hkv, int D, int page_size,
+                                           int max_prefix_pages, int max_pages, int num_pages,
+                                           float scale, bool causal, cudaStream_t stream);
+
 FlashAttentionError launch_lse_merge(float* O_acc, float* L_acc, const float* O_part,
                                      const float* L_part, long long rows, int D,
                                      cudaStream_t stream);

@@ -59,6 +59,12 @@ SIGNATURES = {
     "cuflash_attention_decode_gqa_f16": [_P] * 5 + [_I] * 5 + [_F, _I, _P],
     "cuflash_attention_decode_paged_bf16": [_P] * 7 + [_I] * 7 + [_F, _I, _P],
     "cuflash_attention_decode_paged_f16": [_P] * 7 + [_I] * 7 + [_F, _I, _P],
+    "cuflash_kv_append_paged_bf16": [_P] * 11 + [_I] * 8 + [_LL] * 3 + [_I, _I, _B, _P],
+    "cuflash_kv_append_paged_f16": [_P] * 11 + [_I] * 8 + [_LL] * 3 + [_I, _I, _B, _P],
+    "cuflash_attention_forward_paged_bf16": [_P] * 8 + [_I] * 8 + [_F, _B, _P],
+    "cuflash_attention_forward_paged_f16": [_P] * 8 + [_I] * 8 + [_F, _B, _P],
+    "cuflash_attention_decode_shared_prefix_bf16": [_P] * 9 + [_I] * 8 + [_F, _P],
+    "cuflash_attention_decode_shared_prefix_f16": [_P] * 9 + [_I] * 8 + [_F, _P],
     "cuflash_attention_forward_gqa_bf16": [_P] * 5 + [_I] * 6 + [_F, _B, _P],
     "cuflash_attention_forward_gqa_f16": [_P] * 5 + [_I] * 6 + [_F, _B, _P],
     "cuflash_attention_backward_gqa_bf16": [_P] * 9 + [_I] * 6 + [_F, _B, _P],
@@ -158,6 +164,65 @@ def _stream_handle(stream) -> ctypes.c_void_p:
 
         stream = torch.cuda.current_stream()
     return ctypes.c_void_p(stream.cuda_stream)
+
+
+def rope_table(max_position: int, rotary_dim: int, base: float = 10000.0, device="cuda"):
+    """fp32 [max_position, rotary_dim] for ``kv_append_paged``: the cosines of
+    the angles position * base^(-2i/rotary_dim), then their sines.  Angles are
+    formed in 64 bits: at position 10^5 a 32-bit angle is off by up to 4e-3."""
+    import torch
+
+    half = rotary_dim // 2
+    freq = float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    angle = torch.arange(max_position, dtype=torch.float64)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).to(device, torch.float32)
+
+
+def _token_stride(t) -> int:
+    """Elements between tokens of t [tokens, heads, D] whose heads are packed."""
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError("a token's heads must be contiguous")
+    if t.shape[0] <= 1:
+        return 0
+    if t.stride(0) < t.shape[1] * t.shape[2]:
+        raise ValueError("tokens must not overlap")
+    return t.stride(0)
+
+
+def _check_like(ref, **tensors) -> None:
+    """Same device and dtype as ref."""
+    for name, t in tensors.items():
+        if t.device != ref.device:
+            raise ValueError(f"{name} must be on {ref.device}")
+        if t.dtype != ref.dtype:
+            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {ref.dtype}")
+
+
+def _check_lse(ref, L) -> None:
+    import torch
+
+    if L.dtype != torch.float32 or L.device != ref.device:
+        raise ValueError(f"L must be float32 on {ref.device}")
+
+
+def _check_index(ref, **tensors) -> None:
+    """int32 tensors on ref's device."""
+    import torch
+
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != ref.device:
+            raise ValueError(f"{name} must be on {ref.device}")
+        if t.dtype != torch.int32:
+            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be int32")
+
+
+def _check_shape(**pairs) -> None:
+    for name, (t, shape) in pairs.items():
+        if tuple(t.shape) != tuple(shape):
+            raise CuFlashError(DIMENSION_MISMATCH,
+                               f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
 
 
 class CuFlashAttn:
@@ -276,6 +341,120 @@ class CuFlashAttn:
                             _ptr(seq_lens), _ptr(O), _ptr(L), B, Hq, Hkv, D, page_size,
                             block_table.shape[1], num_pages, float(scale), int(num_splits),
                             _stream_handle(stream)))
+        return O, L
+
+    # The three paged-cache entries below run on the device of their tensors,
+    # whichever device is current, and by default on its current stream.
+    def kv_append_paged(self, K, V, K_cache, V_cache, block_table, seq_lens, cu_seqlens=None,
+                        Q=None, rope_table=None, positions=None, interleaved: bool = False,
+                        Q_out=None, stream=None):
+        """Writes the new tokens' K, V [tokens, Hkv, D] into the paged cache
+        [pages, page_size, Hkv, D] (block_table int32 [B, max_pages], seq_lens
+        int32 [B] with the new tokens, cu_seqlens int32 [B+1] or None for one
+        token per sequence) and rotates Q [tokens, Hq, D] and K by the rows of
+        rope_table (see ``rope_table``) on the way.  Q, K, V may be slices of
+        one projection's output.  Returns Q_out (None without Q)."""
+        import torch
+
+        tokens, Hkv, D = K.shape
+        num_pages, page_size = K_cache.shape[:2]
+        B, max_pages = block_table.shape
+        Hq = 0 if Q is None else Q.shape[1]
+        _check_shape(V=(V, K.shape), K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
+                     V_cache=(V_cache, K_cache.shape), seq_lens=(seq_lens, (B,)))
+        _check_like(K, V=V, K_cache=K_cache, V_cache=V_cache)
+        _check_index(K, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
+                     positions=positions)
+        if cu_seqlens is not None:
+            _check_shape(cu_seqlens=(cu_seqlens, (B + 1,)))
+        if positions is not None:
+            _check_shape(positions=(positions, (tokens,)))
+        if Q is not None:
+            _check_shape(Q=(Q, (tokens, Hq, D)))
+            if Q_out is None:
+                Q_out = torch.empty((tokens, Hq, D), device=Q.device, dtype=Q.dtype)
+            _check_shape(Q_out=(Q_out, Q.shape))
+            _check_like(K, Q=Q, Q_out=Q_out)
+        elif Q_out is not None:
+            raise ValueError("Q_out without Q")
+        max_position = rotary = 0
+        if rope_table is not None:
+            if rope_table.dtype != torch.float32 or rope_table.device != K.device:
+                raise ValueError(f"rope_table must be float32 on {K.device}")
+            max_position, rotary = rope_table.shape
+        strides = [0 if t is None else _token_stride(t) for t in (Q, K, V)]
+        data = [ctypes.c_void_p(0 if t is None else t.data_ptr()) for t in (Q, K, V)]
+        if not K.is_cuda:
+            raise ValueError("tensor must be on a CUDA device")
+        fn = getattr(self.lib, f"cuflash_kv_append_paged_{_suffix(K)}")
+        with torch.cuda.device(K.device):
+            self.check_error(fn(*data, _ptr(Q_out), _ptr(K_cache), _ptr(V_cache),
+                                _ptr(rope_table), _ptr(positions), _ptr(block_table),
+                                _ptr(seq_lens), _ptr(cu_seqlens), tokens, B, Hq, Hkv, D,
+                                page_size, max_pages, num_pages, *strides, rotary, max_position,
+                                bool(interleaved), _stream_handle(stream)))
+        return Q_out
+
+    def forward_paged(self, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens,
+                      causal: bool = True, scale: Optional[float] = None, O=None, L=None,
+                      stream=None):
+        """Ragged attention of the new tokens Q [tokens, Hq, D] (cu_seqlens
+        int32 [B+1]) over their sequences' pages; causal is aligned
+        bottom-right.  Returns O [tokens, Hq, D], L [tokens, Hq]."""
+        import torch
+
+        tokens, Hq, D = Q.shape
+        num_pages, page_size, Hkv, _ = K_cache.shape
+        B, max_pages = block_table.shape
+        if scale is None:
+            scale = 1.0 / math.sqrt(D)
+        O = torch.empty_like(Q) if O is None else O
+        L = torch.empty((tokens, Hq), device=Q.device, dtype=torch.float32) if L is None else L
+        _check_shape(K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
+                     V_cache=(V_cache, K_cache.shape), seq_lens=(seq_lens, (B,)),
+                     cu_seqlens=(cu_seqlens, (B + 1,)), O=(O, Q.shape), L=(L, (tokens, Hq)))
+        _check_like(Q, K_cache=K_cache, V_cache=V_cache, O=O)
+        _check_lse(Q, L)
+        _check_index(Q, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens)
+        fn = getattr(self.lib, f"cuflash_attention_forward_paged_{_suffix(Q)}")
+        with torch.cuda.device(Q.device):
+            self.check_error(fn(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_table),
+                                _ptr(seq_lens), _ptr(cu_seqlens), _ptr(O), _ptr(L), tokens, B,
+                                Hq, Hkv, D, page_size, max_pages, num_pages, float(scale),
+                                bool(causal), _stream_handle(stream)))
+        return O, L
+
+    def decode_shared_prefix(self, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
+                             seq_lens, scale: Optional[float] = None, O=None, L=None,
+                             stream=None):
+        """q [B, Hq, 1, D] against the prefix_len (int32 [1]) keys of the pages
+        prefix_table (int32 [max_prefix_pages]), shared by the batch, and the
+        sequence's own seq_lens[b] keys behind them.  Returns O like q,
+        L [B, Hq]."""
+        import torch
+
+        B, Hq, _, D = q.shape
+        num_pages, page_size, Hkv, _ = K_cache.shape
+        max_pages = block_table.shape[1]
+        if scale is None:
+            scale = 1.0 / math.sqrt(D)
+        O = torch.empty_like(q) if O is None else O
+        L = torch.empty((B, Hq), device=q.device, dtype=torch.float32) if L is None else L
+        _check_shape(q=(q, (B, Hq, 1, D)), K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
+                     V_cache=(V_cache, K_cache.shape), prefix_len=(prefix_len, (1,)),
+                     prefix_table=(prefix_table, (prefix_table.numel(),)),
+                     block_table=(block_table, (B, max_pages)), seq_lens=(seq_lens, (B,)),
+                     O=(O, q.shape), L=(L, (B, Hq)))
+        _check_like(q, K_cache=K_cache, V_cache=V_cache, O=O)
+        _check_lse(q, L)
+        _check_index(q, prefix_table=prefix_table, prefix_len=prefix_len,
+                     block_table=block_table, seq_lens=seq_lens)
+        fn = getattr(self.lib, f"cuflash_attention_decode_shared_prefix_{_suffix(q)}")
+        with torch.cuda.device(q.device):
+            self.check_error(fn(_ptr(q), _ptr(K_cache), _ptr(V_cache), _ptr(prefix_table),
+                                _ptr(prefix_len), _ptr(block_table), _ptr(seq_lens), _ptr(O),
+                                _ptr(L), B, Hq, Hkv, D, page_size, prefix_table.numel(),
+                                max_pages, num_pages, float(scale), _stream_handle(stream)))
         return O, L
 
     def forward_gqa(self, Q, K, V, causal: bool = False, scale: Optional[float] = None, O=None,

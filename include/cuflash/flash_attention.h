@@ -235,6 +235,84 @@ CUFLASH_EXPORT int cuflash_attention_decode_paged_f16(
     int head_dim, int page_size, int max_pages_per_seq, int num_pages, float scale,
     int num_splits, cudaStream_t stream);
 
+// Serving over a paged KV cache (no reference counterpart).  The cache, the
+// block table, the page clamping and the head grouping are those of
+// cuflash_attention_decode_paged_*; pool and table must address fewer than
+// 2^31 rows.  All tables, lengths and positions are int32 in device memory,
+// read when the kernels run, so a captured graph sees their values at replay.
+//
+// Append: the batch's new tokens, packed one sequence after the other, enter
+// the cache.  Q [num_tokens, num_q_heads, D], K, V [num_tokens, num_kv_heads,
+// D]; the strides are elements between tokens (0: contiguous; else a multiple
+// of 8 and at least the token's heads), so the three may be slices of one
+// projection's output.  cu_seqlens [B+1] ascends from 0: tokens cu_seqlens[b]
+// .. cu_seqlens[b+1]-1 are the last ones of sequence b, whose length with
+// them is seq_lens[b] (what the attention entries take next); NULL: token b
+// is the only one of sequence b (num_tokens == batch_size).  K and V rows go to
+// page block_table[b][i / page_size], slot i % page_size for the token's
+// index i; a token whose index is negative or behind the table, or whose page
+// is outside [0, num_pages), is not stored.  Two tokens must not share a place.
+// rope_table fp32 [max_position, rotary_dim] (cosines of the rotary_dim/2
+// angles, then sines; NULL: no rotation): Q and K are rotated by the row of
+// positions[t] (NULL: the token's index), clamped to the table, in fp32 and
+// rounded once.  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) with
+// interleaved; elements from rotary_dim on pass through.  rotary_dim is a
+// multiple of 16.  The rotated queries go to Q_out [num_tokens, num_q_heads,
+// D] contiguous (may be Q itself where Q is contiguous; Q and Q_out both NULL:
+// keys and values only).  Tokens from cu_seqlens[B] on are left alone.
+CUFLASH_EXPORT int cuflash_kv_append_paged_bf16(
+    const __nv_bfloat16* Q, const __nv_bfloat16* K, const __nv_bfloat16* V, __nv_bfloat16* Q_out,
+    __nv_bfloat16* K_cache, __nv_bfloat16* V_cache, const float* rope_table, const int* positions,
+    const int* block_table, const int* seq_lens, const int* cu_seqlens, int num_tokens,
+    int batch_size, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+    int max_pages_per_seq, int num_pages, long long q_stride, long long k_stride,
+    long long v_stride, int rotary_dim, int max_position, bool interleaved, cudaStream_t stream);
+CUFLASH_EXPORT int cuflash_kv_append_paged_f16(
+    const half* Q, const half* K, const half* V, half* Q_out, half* K_cache, half* V_cache,
+    const float* rope_table, const int* positions, const int* block_table, const int* seq_lens,
+    const int* cu_seqlens, int num_tokens, int batch_size, int num_q_heads, int num_kv_heads,
+    int head_dim, int page_size, int max_pages_per_seq, int num_pages, long long q_stride,
+    long long k_stride, long long v_stride, int rotary_dim, int max_position, bool interleaved,
+    cudaStream_t stream);
+
+// Ragged forward over the paged cache: the new tokens' queries Q, O
+// [num_tokens, num_q_heads, D], L fp32 [num_tokens, num_q_heads], packed by
+// cu_seqlens as in the append (whose keys are already in the cache), against
+// the seq_lens[b] keys of their sequence.  causal aligns bottom-right: token i
+// of the n new ones sees key j iff j <= i + seq_lens[b] - n.  A token that sees
+// no key gets O = 0 and L = -inf; rows from cu_seqlens[B] on are left as they
+// were.  Sequences may have any number of new tokens, none included, so one
+// call serves prompts, chunks of prompts and single tokens together.
+CUFLASH_EXPORT int cuflash_attention_forward_paged_bf16(
+    const __nv_bfloat16* Q, const __nv_bfloat16* K_cache, const __nv_bfloat16* V_cache,
+    const int* block_table, const int* seq_lens, const int* cu_seqlens, __nv_bfloat16* O, float* L,
+    int num_tokens, int batch_size, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+    int max_pages_per_seq, int num_pages, float scale, bool causal, cudaStream_t stream);
+CUFLASH_EXPORT int cuflash_attention_forward_paged_f16(
+    const half* Q, const half* K_cache, const half* V_cache, const int* block_table,
+    const int* seq_lens, const int* cu_seqlens, half* O, float* L, int num_tokens, int batch_size,
+    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages_per_seq,
+    int num_pages, float scale, bool causal, cudaStream_t stream);
+
+// Decode behind a shared prefix: one query token per sequence (Q, O
+// [B, num_q_heads, 1, D], L fp32 [B, num_q_heads]) against the prefix_len[0]
+// keys of the pages prefix_table [max_prefix_pages], which every sequence of
+// the batch shares and which are read once for all of them, followed by the
+// sequence's own seq_lens[b] keys (0 or more) of block_table[b].  The result is
+// that of attention over both together; neither any prefix nor own key: O = 0
+// and L = -inf.
+CUFLASH_EXPORT int cuflash_attention_decode_shared_prefix_bf16(
+    const __nv_bfloat16* Q, const __nv_bfloat16* K_cache, const __nv_bfloat16* V_cache,
+    const int* prefix_table, const int* prefix_len, const int* block_table, const int* seq_lens,
+    __nv_bfloat16* O, float* L, int batch_size, int num_q_heads, int num_kv_heads, int head_dim,
+    int page_size, int max_prefix_pages, int max_pages_per_seq, int num_pages, float scale,
+    cudaStream_t stream);
+CUFLASH_EXPORT int cuflash_attention_decode_shared_prefix_f16(
+    const half* Q, const half* K_cache, const half* V_cache, const int* prefix_table,
+    const int* prefix_len, const int* block_table, const int* seq_lens, half* O, float* L,
+    int batch_size, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+    int max_prefix_pages, int max_pages_per_seq, int num_pages, float scale, cudaStream_t stream);
+
 // Grouped-query (GQA / MQA) attention with separate query and key lengths
 // (no reference counterpart: the reference API has one seq_len and equal
 // head counts).  Q, O, dO, dQ [B, num_q_heads, seq_len_q, D]; K, V, dK, dV
