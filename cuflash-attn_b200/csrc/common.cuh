@@ -255,6 +255,7 @@ int bwd_sm100_status();
 int dec_sm100_status();
 int f32_sm100_status();
 int bwd_f32_sm100_status();
+int paged_sm100_status();
 
 }  // namespace detail
 }  // namespace cuflash

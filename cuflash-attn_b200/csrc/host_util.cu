@@ -394,14 +394,15 @@ int read_and_clear_device_status() {
     const int c = f32_sm100_status();
     const int d = dec_sm100_status();
     const int e = bwd_f32_sm100_status();
-    if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
+    const int f = paged_sm100_status();
+    if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0) return -1;
     const int h = host_status();
     int dev = 0;
     HostStatus* blk = g_host_status.load(std::memory_order_acquire);
     if (blk != nullptr && cudaGetDevice(&dev) == cudaSuccess && dev >= 0 &&
         dev < kMaxStatusDevices)
         *reinterpret_cast<volatile int*>(&blk->word[dev]) = 0;
-    for (const int v : {a, b, c, d, e, h})
+    for (const int v : {a, b, c, d, e, f, h})
         if (v != 0) return v;
     return 0;
 }
