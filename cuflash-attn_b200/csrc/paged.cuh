@@ -13,6 +13,7 @@ __host__ __device__ __forceinline__ int clamp_len(int n, int most) {
     return n < 0 ? 0 : (n < most ? n : most);
 }
 
+#ifdef __CUDACC__
 // Sequence of token t among cu[0..B] (ascending, cu[b] = first token of
 // sequence b): the last b with cu[b] <= t < cu[b + 1], or -1 for a token
 // outside [cu[0], cu[B]).  Each round the 32 lanes probe 32 evenly spaced
@@ -35,6 +36,7 @@ __device__ __forceinline__ int sequence_of_token(const int* __restrict__ cu, int
     }
     return lo;
 }
+#endif
 
 }  // namespace detail
 }  // namespace cuflash

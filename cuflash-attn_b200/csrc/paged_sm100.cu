@@ -10,6 +10,7 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_line.cuh"
 
 namespace cuflash {
 namespace detail {
@@ -180,45 +181,43 @@ FlashAttentionError paged_row(const PagedParams<T>& p, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------
-// Tensor-core kernel (pages of 8 rows and more).
-//
-// Work.  A context is a run of query tokens with one key sequence: sequence b
-// (ragged), or the shared prefix with every sequence's token, and each
-// sequence's own keys with its one token (prefix decode).  The query heads of
-// one K/V head are packed with the tokens into row tiles of M = 128 (tpt tokens
-// x gt heads), so K/V rows are read once for all of them.  A unit is one K/V
-// head (and chunk of gt <= 128 query heads) with two row tiles, or one where
-// no second is left; its length is its number of 128-key blocks.  All units'
-// blocks, one after the other, form a line that is cut into equal pieces, one
-// per CTA: lengths live in device memory, so every CTA sums the contexts'
-// lengths itself and finds its piece.  A piece that covers a unit writes the
-// result; other pieces write normalised fp32 partials with their
-// log2-sum-exp, joined by a second kernel in a fixed order.
-//
-// CTA.  Two streams of 128 softmax threads (one per row) take the steps
-// (row tile x key block) in turn, so one stream's softmax runs under the
-// other's products:
-//   two tiles:  tile 0 and tile 1 of the same block (K/V staged once);
-//   one tile:   alternate blocks of the same tile, each stream with its own
-//               maximum, sum and output; the stream that had the first block
-//               joins both from TMEM at the end of the piece.
-//   warp 0      TMA producer (query tiles, K/V blocks through a ring of
-//               slots, one box per page and 64 columns, one lane each)
+// Tensor-core kernel (pages of 8 rows and more); paged_line.cuh says how the
+// work is divided.  One CTA per SM walks its segments (its parts of units).
+// Two streams of 128 softmax threads take the steps in turn, so that one
+// stream's softmax runs under the other's products:
+//   two tiles:  row tile 0 and row tile 1 of the same key block, a thread per
+//               row: S = Q K^T (M = N = 128), P over S in TMEM, O += P V;
+//   one tile:   the same with alternate blocks of the one tile, each stream
+//               with its own maximum, sum and output; the stream that had the
+//               first block joins both from TMEM at the segment's end;
+//   few rows:   alternate blocks too, but transposed, a thread per key:
+//               S^T = K Q^T (M = 128 keys, N = 16 rows), P^T through shared
+//               memory, O^T += V^T P^T (M = head_dim).  A thread of the tile
+//               forms evaluates 128 exponentials per block however few rows
+//               are live (8 cycles each on the MUFU pipe of its quarter);
+//               here 128 threads on four quarters share them, and the result's
+//               rows lie across the lanes, so they are stored coalesced.
+//   warp 0      TMA producer: query tiles, K/V blocks through a ring of
+//               slots, one box per page and 64 columns, one lane each
 //   warp 1      tcgen05.mma issuer: S(n+2) behind O(n)
-//   warp 2      walks the units and hands out segment descriptors
+//   warp 2      walks the line and hands out segments
 //   warps 4-11  softmax and epilogue
-// S_t = Q K^T (M = N = 128) in TMEM columns [128 t, +128), P_t in 16 bits over
-// its first half, O_t += P V in [256 + 128 t, +D).  Arithmetic as in the dense
-// forward: fp32 statistics in the log2 domain, O rescaled only where a row's
-// maximum grows by more than 2^8, P rounded to the input type for its product.
+// TMEM: S_t in columns [128 t, +128), O_t in [256 + 128 t, +D).  Arithmetic as
+// in the dense forward: fp32 statistics in the log2 domain, O rescaled only
+// where a row's maximum grows by more than 2^8, P rounded to the input type
+// for its product, O accumulated in fp32.
+//
+// Partials (normalised fp32 rows with their log2-sum-exp) are kept as
+// [D/4][rows][4], so that a warp of row-per-lane threads stores and loads 512
+// contiguous bytes (row-major, its 16-byte pieces lie 4 D bytes apart: 3.3 us
+// against 0.9 us for a 128-row tile of D = 128).
 // ---------------------------------------------------------------------------
 __device__ sm100::StatusWord g_paged_status;
 
 constexpr int kTcThreads = 384;
 constexpr int kSegRing = 4;
-constexpr int kTileRows = 128;
-constexpr int kBlockKeys = 128;
 constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kFewRows = 16;      // N of the transposed products
 
 template <int D>
 struct PagedGeom {
@@ -228,275 +227,46 @@ struct PagedGeom {
     static constexpr int kNumCb = D / kCbElems;
     static constexpr int kCbBytes = kTileRows * kSwz;
     static constexpr int kTileBytes = kTileRows * kRowBytes;
+    // the transposed form is not built for 64-byte rows (head_dim 32)
+    static constexpr bool kHasFew = D >= 64;
     // K and V blocks share one ring; at D = 128 five slots of 32 KB fill what
     // the two query tiles leave
-    static constexpr int kSlots = D == 128 ? 5 : (D == 64 ? 10 : 12);
+    static constexpr int kSlots = D == 128 ? 5 : (D == 64 ? 9 : 12);
     static constexpr uint32_t kLayout = kSwz == 128 ? sm100::kLayoutSw128 : sm100::kLayoutSw64;
-    static constexpr int kOffRing = 2 * kTileBytes;
-    static constexpr int kOffMl = kOffRing + kSlots * kTileBytes;  // 128 x (maximum, sum)
+    // Few rows: a query slot holds the 16 query rows at the start of each
+    // column block, and in between, from 4 KB on, each stream's P^T (two
+    // 64-key column blocks of 16 rows) and the exchange of block maxima; it is
+    // released when the segment's last product has read P^T.
+    static constexpr int kQSlotBytes = kTileBytes < 16384 ? 16384 : kTileBytes;
+    static constexpr int kOffPt = 4096;
+    static constexpr int kPtBytes = 2 * kFewRows * 128;
+    static constexpr int kOffMax = kOffPt + 2 * kPtBytes;  // [2 streams][2][4 warps][16]
+    static constexpr int kOffRing = 2 * kQSlotBytes;
+    // the transposed value product reads 128 columns from every slot; at D = 64
+    // the upper 64 are the next slot's (rows of O^T nobody reads), so the last
+    // slot is followed by as many bytes
+    static constexpr int kPad = kHasFew ? 128 * 256 - kTileBytes : 0;
+    static constexpr int kOffMl = kOffRing + kSlots * kTileBytes + kPad;
     static constexpr int kOffSeg = kOffMl + kTileRows * 8;
-    static constexpr int kOffScan = kOffSeg + kSegRing * 48;  // 12 warp sums, context, its start
-    static constexpr int kOffBar = kOffScan + 12 * 8 + 16;
-    static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 4 * 2 + 2 + 2 * kSegRing + 1;
+    static constexpr int kOffScan = kOffSeg + kSegRing * static_cast<int>(sizeof(Seg));
+    static constexpr int kOffBar = kOffScan + 96;  // 12 warp sums, start context
+    static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 5 * 2 + 2 + 2 * kSegRing + 1;
     static constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;
     static_assert(kOffBar % 8 == 0 && kSmemBytes <= 232448, "shared memory layout");
 };
 
-// What the roles need to know about one CTA's part of one unit.
-struct Seg {
-    int n_blk;     // key blocks; 0 ends the CTA's work
-    int blk0;      // first key block
-    int len;       // keys of the context
-    int lim0;      // causal: last key the first token of tile 0 sees
-    int tok0;      // first token of tile 0
-    int tok_end;   // end of the context's tokens
-    int head0;     // first query head
-    int nh;        // query heads
-    int hk;        // K/V head
-    int ctx;       // sequence, or -1 for the shared prefix
-    int two;       // two row tiles
-    int part_row;  // first partial row, -1: the whole unit, write the result
-};
-static_assert(sizeof(Seg) == 48, "Seg layout");
-
-// A unit whose blocks several CTAs share (ragged): written by the first.
-struct Split {
-    int last;  // last CTA of the unit, -1: none
-    int tok0, tok_end, head0, nh, two;
-    int pad[2];
-};
-
 struct TcParams {
+    PagedLine ln;
     void* O;
     float* L;
     float* O_part;
-    float* L_part;          // log2-sum-exp of each partial row
-    long long* per;         // blocks per CTA, for the second kernel
-    long long* unit_start;  // prefix decode: line position of each own-keys unit
-    Split* split;           // ragged: per CTA
+    float* L_part;  // log2-sum-exp of each partial row
     const int* prefix_table;
-    const int* prefix_len;
     const int* block_table;
-    const int* seq_lens;
-    const int* cu_seqlens;
-    int prefix_mode;
-    int num_tokens, B, hq, hkv, group;
-    int gt, chunks, tpt;  // heads per tile, chunks of the group, tokens per tile
-    int page_shift, max_prefix_pages, max_pages, num_pages;
-    int causal;
-    int w_two, w_one;  // line length of a block of a two-tile and of a one-tile unit
-    int min_per;
-    long long own_part_row;  // first partial row of the own-keys units
+    int few_tok;  // tokens of the few-rows query box
+    int num_pages;
     float scale_log2;
 };
-
-// sum over i in [0, n) of floor((a i + b) / m): the usual Euclid-like
-// reduction (a, b >= 0, m > 0).
-__host__ __device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-    long long s = 0;
-    while (n > 0) {
-        s += (n * (n - 1) / 2) * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const long long top = a * n + b;
-        n = top / m;
-        b = top % m;
-        const long long t = m;
-        m = a;
-        a = t;
-        if (m == 0) break;  // then top < the old m and n == 0
-    }
-    return s;
-}
-
-struct Ctx {
-    int tok, ntok, len;
-    int pairs;       // units per head chunk
-    int last_two;    // the last unit has two tiles
-    long long head_cost;
-};
-
-__host__ __device__ __forceinline__ int unit_blocks(const TcParams& p, const Ctx& c, int pair) {
-    int vis = c.len;
-    if (p.causal && pair < c.pairs - 1)
-        vis = c.len - c.ntok + (pair + 1) * 2 * p.tpt;  // what its last token sees
-    const int nb = (vis + kBlockKeys - 1) / kBlockKeys;
-    // ragged: a unit that sees no key takes one masked block, which writes its rows
-    return p.prefix_mode ? nb : (vis > 0 ? nb : 1);
-}
-
-__host__ __device__ __forceinline__ int unit_weight(const TcParams& p, const Ctx& c, int pair) {
-    return pair < c.pairs - 1 || c.last_two ? p.w_two : p.w_one;
-}
-
-// Line length of the first `pairs` units (of two tiles each) of a head chunk.
-__host__ __device__ __forceinline__ long long pairs_cost(const TcParams& p, const Ctx& c, int pairs) {
-    if (!p.causal) return static_cast<long long>(pairs) * unit_blocks(p, c, 0) * p.w_two;
-    const int s = 2 * p.tpt;
-    const int off = c.len - c.ntok;
-    // units whose last token sees at most 128 keys take one block
-    int ones = 128 - off >= 0 ? (128 - off) / s : 0;
-    if (ones > pairs) ones = pairs;
-    return (ones + floor_sum(pairs - ones, 128, s,
-                             static_cast<long long>(off) + static_cast<long long>(ones + 1) * s + 127)) *
-           p.w_two;
-}
-
-// Context c: -1 is the shared prefix.
-__host__ __device__ __forceinline__ Ctx load_ctx(const TcParams& p, int c) {
-    Ctx x;
-    if (p.prefix_mode) {
-        x.tok = c < 0 ? 0 : c;
-        x.ntok = c < 0 ? p.B : 1;
-        x.len = c < 0 ? clamp_len(*p.prefix_len, p.max_prefix_pages << p.page_shift)
-                      : clamp_len(p.seq_lens[c], p.max_pages << p.page_shift);
-    } else {
-        x.tok = clamp_len(p.cu_seqlens[c], p.num_tokens);
-        x.ntok = clamp_len(p.cu_seqlens[c + 1] - x.tok, p.num_tokens - x.tok);
-        x.len = clamp_len(p.seq_lens[c], p.max_pages << p.page_shift);
-    }
-    const int tiles = (x.ntok + p.tpt - 1) / p.tpt;
-    x.pairs = (tiles + 1) / 2;
-    x.last_two = (tiles & 1) == 0;
-    x.head_cost = 0;
-    if (x.pairs > 0 && (x.len > 0 || !p.prefix_mode))
-        x.head_cost = pairs_cost(p, x, x.pairs - 1) +
-                      static_cast<long long>(unit_blocks(p, x, x.pairs - 1)) *
-                          unit_weight(p, x, x.pairs - 1);
-    return x;
-}
-
-// The piece [x0, x1) of the line that belongs to CTA `cta`, unit by unit.
-struct Walk {
-    Ctx ctx;
-    int c, hc, pair, cta;  // context, head chunk, unit of it
-    long long ub, x, x1, per;  // line position of the unit, of the walk, its end
-};
-
-// Context c holds position x0 and starts at ctx_base.
-__host__ __device__ __forceinline__ void walk_start(const TcParams& p, Walk& w, int c,
-                                                    long long ctx_base, long long x0, long long x1,
-                                                    long long per, int cta) {
-    w.ctx = load_ctx(p, c);
-    w.c = c;
-    w.cta = cta;
-    w.x = x0;
-    w.x1 = x1;
-    w.per = per;
-    long long y = x0 - ctx_base;
-    w.hc = static_cast<int>(y / w.ctx.head_cost);
-    y -= w.hc * w.ctx.head_cost;
-    int lo = 0, hi = w.ctx.pairs;  // the unit of the head chunk that y falls into
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (pairs_cost(p, w.ctx, mid) <= y)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    w.pair = lo;
-    w.ub = ctx_base + w.hc * w.ctx.head_cost + pairs_cost(p, w.ctx, lo);
-}
-
-// The next segment; false at the end.  Records where units start (own keys)
-// and which units several CTAs share (ragged) for the second kernel.
-__host__ __device__ __forceinline__ bool walk_next(const TcParams& p, Walk& w, Seg& sg) {
-    const int heads = p.hkv * p.chunks;
-    while (w.x < w.x1) {
-        const int nb = unit_blocks(p, w.ctx, w.pair);
-        const int wt = unit_weight(p, w.ctx, w.pair);
-        const int blk0 = static_cast<int>((w.x - w.ub + wt - 1) / wt);
-        const long long end = (w.x1 - w.ub + wt - 1) / wt;
-        const int blk1 = end < nb ? static_cast<int>(end) : nb;
-        const bool some = blk1 > blk0;
-        if (some) {
-            sg.n_blk = blk1 - blk0;
-            sg.blk0 = blk0;
-            sg.len = w.ctx.len;
-            sg.lim0 = w.ctx.len - w.ctx.ntok + w.pair * 2 * p.tpt;
-            sg.tok0 = w.ctx.tok + w.pair * 2 * p.tpt;
-            sg.tok_end = w.ctx.tok + w.ctx.ntok;
-            sg.hk = w.hc / p.chunks;
-            const int ch = w.hc - sg.hk * p.chunks;
-            sg.head0 = sg.hk * p.group + ch * p.gt;
-            sg.nh = p.group - ch * p.gt < p.gt ? p.group - ch * p.gt : p.gt;
-            sg.ctx = w.c;
-            sg.two = w.pair < w.ctx.pairs - 1 || w.ctx.last_two;
-            if (p.prefix_mode) {
-                if (w.c < 0) {
-                    sg.part_row = (w.hc * w.ctx.pairs + w.pair + w.cta) * (2 * kTileRows);
-                } else {
-                    const long long u = static_cast<long long>(w.c) * heads + w.hc;
-                    if (blk0 == 0) p.unit_start[u] = w.ub;
-                    sg.part_row = static_cast<int>(p.own_part_row + (u + w.cta) * p.gt);
-                }
-            } else if (blk0 == 0 && blk1 == nb) {
-                sg.part_row = -1;
-            } else {
-                sg.part_row = (2 * w.cta + (blk0 == 0 ? 1 : 0)) * (2 * kTileRows);
-                if (blk0 == 0) {
-                    Split sp;
-                    sp.last = static_cast<int>((w.ub + static_cast<long long>(nb - 1) * wt) / w.per);
-                    sp.tok0 = sg.tok0;
-                    sp.tok_end = sg.tok_end;
-                    sp.head0 = sg.head0;
-                    sp.nh = sg.nh;
-                    sp.two = sg.two;
-                    p.split[w.cta] = sp;
-                }
-            }
-        }
-        w.ub += static_cast<long long>(nb) * wt;
-        w.x = w.ub;
-        if (++w.pair == w.ctx.pairs) {
-            w.pair = 0;
-            if (++w.hc == heads) {
-                w.hc = 0;
-                while (w.x < w.x1 && w.c < p.B - 1) {
-                    w.ctx = load_ctx(p, ++w.c);
-                    if (w.ctx.head_cost != 0) break;
-                }
-            }
-        }
-        if (some) return true;
-    }
-    return false;
-}
-
-// Partials of the output row (sequence b, query head h): n1 rows from row1 on,
-// 2 kTileRows apart (the prefix), and n2 rows from row2 on, gt apart (own keys).
-struct PrefixParts {
-    int n1, n2;
-    long long row1, row2;
-};
-
-__host__ __device__ __forceinline__ PrefixParts prefix_parts(const TcParams& p, const Ctx& pre,
-                                                             const Ctx& own, int b, int h) {
-    PrefixParts q = {0, 0, 0, 0};
-    const long long per = *p.per;
-    const int hk = h / p.group, hg = h - hk * p.group;
-    const int ch = hg / p.gt, hr = hg - ch * p.gt;
-    const int hc = hk * p.chunks + ch;
-    if (pre.len > 0) {
-        const int tile = b / p.tpt;
-        const int pair = tile >> 1;
-        const long long nb = unit_blocks(p, pre, pair);
-        const long long ub = hc * pre.head_cost + pairs_cost(p, pre, pair);
-        const long long i0 = ub / per;
-        q.n1 = static_cast<int>((ub + (nb - 1) * unit_weight(p, pre, pair)) / per - i0) + 1;
-        q.row1 = (static_cast<long long>(hc) * pre.pairs + pair + i0) * (2 * kTileRows) +
-                 (tile & 1) * kTileRows + (b - tile * p.tpt) * p.gt + hr;
-    }
-    if (own.len > 0) {
-        const long long u = static_cast<long long>(b) * p.hkv * p.chunks + hc;
-        const long long nb = unit_blocks(p, own, 0);
-        const long long ub = p.unit_start[u];
-        const long long i0 = ub / per;
-        q.n2 = static_cast<int>((ub + (nb - 1) * p.w_one) / per - i0) + 1;
-        q.row2 = p.own_part_row + (u + i0) * p.gt + hr;
-    }
-    return q;
-}
 
 template <int D>
 __device__ __forceinline__ uint64_t pg_kdesc(uint32_t base) {  // K-major, k-step 0
@@ -518,41 +288,82 @@ template <int D>
 __host__ __device__ constexpr uint32_t pg_vdelta(int kk) {
     return (static_cast<uint32_t>(kk) * 16u * PagedGeom<D>::kSwz) >> 4;
 }
+// P^T, K-major: [2 blocks of 64 keys][16 rows][128 bytes]
+__host__ __device__ constexpr uint32_t pt_delta(int kk) {
+    return (static_cast<uint32_t>(kk >> 2) * (kFewRows * 128) + static_cast<uint32_t>(kk & 3) * 32u) >> 4;
+}
 
-template <typename T, int D>
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(sm100::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+
+// NC: columns of the few-rows form (contexts of more rows take row tiles).
+template <typename T, int D, int NC>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQf,
                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                      const TcParams p) {
+                      const __grid_constant__ TcParams p) {
     using G = PagedGeom<D>;
     using namespace sm100;
     constexpr int R = G::kSlots;
     extern __shared__ uint8_t smem_raw[];
+    const PagedLine& ln = p.ln;
+    // the joining kernel's blocks may wait on the SMs this one leaves
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (cta_skip(&g_paged_status)) return;
+
+    // ---- this thread's contexts (first: their loads are the longest latency)
+    const int c_lo = ln.prefix_mode ? -1 : 0;
+    const int n_ctx = ln.B - c_lo;
+    const int heads = ln.hkv * ln.chunks;
+    const int run = (n_ctx + kTcThreads - 1) / kTcThreads;  // contexts per thread
+    const int c_first = c_lo + min(static_cast<int>(threadIdx.x) * run, n_ctx);
+    const int c_last = min(c_first + run, ln.B);
+    Ctx ctx1 = {};
+    int mine = 0;
+    for (int c = c_first; c < c_last; ++c) {
+        ctx1 = load_ctx(ln, c);
+        mine += ctx1.head_cost * heads;
+    }
 
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     uint8_t* sptr = smem_raw + (sbase - raw);
     uint64_t* bar_q = reinterpret_cast<uint64_t*>(sptr + G::kOffBar);  // [2] query tile landed
-    uint64_t* bar_qfree = bar_q + 2;      // [2] its last product retired
+    uint64_t* bar_qfree = bar_q + 2;      // [2] its slot is free
     uint64_t* full = bar_qfree + 2;       // [R]
     uint64_t* empty = full + R;           // [R]
     uint64_t* bar_s = empty + R;          // [2] S_t in TMEM
-    uint64_t* bar_p = bar_s + 2;          // [2] first half of P_t stored
+    uint64_t* bar_p = bar_s + 2;          // [2] first half of P_t (few rows: P_t) stored
     uint64_t* bar_p2 = bar_p + 2;         // [2] second half
     uint64_t* bar_o = bar_p2 + 2;         // [2] O_t final for the segment
-    uint64_t* bar_x = bar_o + 2;          // one tile: second stream's state is there
-    uint64_t* bar_y = bar_x + 1;          // one tile: it has been read
+    uint64_t* bar_m = bar_o + 2;          // [2] few rows: the stream's warps have exchanged
+    uint64_t* bar_x = bar_m + 2;          // second stream's state is there
+    uint64_t* bar_y = bar_x + 1;          // it has been read
     uint64_t* seg_full = bar_y + 1;       // [kSegRing]
     uint64_t* seg_free = seg_full + kSegRing;  // [kSegRing]
     uint64_t* bar_done = seg_free + kSegRing;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Seg* segs = reinterpret_cast<Seg*>(sptr + G::kOffSeg);
-    long long* scan = reinterpret_cast<long long*>(sptr + G::kOffScan);  // [12]
-    long long* first_base = scan + 12;  // line position of the context the CTA starts in
-    int* first_ctx = reinterpret_cast<int*>(scan + 13);
+    int* scan = reinterpret_cast<int*>(sptr + G::kOffScan);  // [12] warp sums
+    int* start_c = scan + 12;     // context the piece starts in, -2: none
+    int* start_base = scan + 13;  // its line position
+    Ctx* start_ctx = reinterpret_cast<Ctx*>(scan + 14);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -565,6 +376,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(bar_p + t, 128);
             mbar_init(bar_p2 + t, 128);
             mbar_init(bar_o + t, 1);
+            mbar_init(bar_m + t, 4);
         }
         for (int s = 0; s < R; ++s) {
             mbar_init(full + s, 1);
@@ -578,7 +390,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
-        *first_ctx = -2;
+        *start_c = -2;
+        if (!ln.prefix_mode) ln.split[blockIdx.x].last = -1;
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
+        prefetch_tmap(&tmQ);
+        prefetch_tmap(&tmQf);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -587,56 +404,58 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 
     // ---- the line: contexts' lengths summed over the block
-    const int c_lo = p.prefix_mode ? -1 : 0;
-    const int n_ctx = p.B - c_lo;
-    const long long heads = static_cast<long long>(p.hkv) * p.chunks;
-    const int run = (n_ctx + kTcThreads - 1) / kTcThreads;  // contexts per thread
-    const int c_first = c_lo + static_cast<int>(min(static_cast<long long>(threadIdx.x) * run,
-                                                    static_cast<long long>(n_ctx)));
-    const int c_last = min(c_first + run, p.B);
-    long long mine = 0;
-    for (int c = c_first; c < c_last; ++c) mine += load_ctx(p, c).head_cost * heads;
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
         if (lane >= off) incl += v;
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kTcThreads / 32; ++w) {
-        const long long v = scan[w];
+        const int v = scan[w];
         if (w < warp) before += v;
         total += v;
     }
-    long long per = (total + gridDim.x - 1) / gridDim.x;
-    if (per < p.min_per) per = p.min_per;
-    const long long x0 = static_cast<long long>(blockIdx.x) * per;
-    const long long x1 = min(x0 + per, total);
+    const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), ln.min_per);
+    const int x0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
+    const int x1 = min(x0 + per, total);
     {
-        long long base = before + incl - mine;
-        if (x0 >= base && x0 < base + mine) {
+        int base = before + incl - mine;
+        if (x0 < x1 && x0 >= base && x0 < base + mine) {
             for (int c = c_first; c < c_last; ++c) {
-                const long long cost = load_ctx(p, c).head_cost * heads;
+                if (run > 1) ctx1 = load_ctx(ln, c);
+                const int cost = ctx1.head_cost * heads;
                 if (x0 < base + cost) {
-                    *first_ctx = c;
-                    *first_base = base;
+                    *start_c = c;
+                    *start_base = base;
+                    *start_ctx = ctx1;
                     break;
                 }
                 base += cost;
             }
         }
     }
-    if (threadIdx.x == 0) {
-        if (blockIdx.x == 0) *p.per = per;
-        if (!p.prefix_mode) p.split[blockIdx.x].last = -1;
-    }
+    if (threadIdx.x == 0 && blockIdx.x == 0) *ln.per = per;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+
+    // Bounded waits, short enough to be inlined everywhere: a wait gives up
+    // when the role's segment has lasted the limit or another role has given up; the role that ran out records it on its way out.
+    bool ok = true;
+    auto tick = [] { return static_cast<uint32_t>(globaltimer_ns() >> 10); };  // about 1 us
+    constexpr uint32_t kWaitTicks = static_cast<uint32_t>(kWaitTimeoutNs >> 10);
+    uint32_t since = tick();
+    auto poll = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const uint32_t addr = smem_u32(bar);
+        while (!mbar_try_wait(addr, parity))
+            if (*abort_flag || tick() - since > kWaitTicks) return false;
+        return true;
+    };
 
     // Registers: launched with 168 per thread (384 x 168 = 64512); the first
     // warpgroup gives back down to 72 and the two softmax warpgroups take 216:
@@ -647,69 +466,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ------------------------------------------------ TMA producer
             uint32_t q_cnt[2] = {0u, 0u};
             uint32_t kv = 0;  // ring fills
-            int qs = 0;       // query slot of the next one-tile segment
-            const int box_rows = min(1 << p.page_shift, kBlockKeys);
+            int qs = 0;       // query slot of the next segment of one tile
+            const int box_rows = min(1 << ln.page_shift, kBlockKeys);
             const int boxes = kBlockKeys / box_rows;  // per block and column block, <= 16
             const int my_box = lane & 15;
             const int my_cb = lane >> 4;
-            bool ok = true;
-            if (lane == 0) {
-                prefetch_tmap(&tmQ);
-                prefetch_tmap(&tmQ1);
-                prefetch_tmap(&tmK);
-                prefetch_tmap(&tmV);
-            }
+            // Table entries come 32 boxes at a time, one per lane, a chunk ahead
+            // (and the first of the next segment with this one's last block), so
+            // that no copy waits for its page's index.
+            auto load_entry = [&](const Seg& sg, int chunk) -> int {
+                const int* table = sg.ctx < 0 ? p.prefix_table
+                                              : p.block_table + static_cast<long long>(sg.ctx) * ln.max_pages;
+                const long long row = (static_cast<long long>(chunk) * 32 + lane) * box_rows;
+                return row < sg.len ? table[row >> ln.page_shift] : 0;
+            };
+            int entry_next_seg = 0;
+            bool have_next = false;
             for (int k = 0;; ++k) {
-                ok = mbar_wait(seg_full + k % kSegRing, (k / kSegRing) & 1, abort_flag, &g_paged_status);
+                ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const Seg sg = segs[k % kSegRing];
                 __syncwarp();
                 if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
                 if (sg.n_blk == 0) break;
-                const int* table = sg.ctx < 0 ? p.prefix_table
-                                              : p.block_table + static_cast<long long>(sg.ctx) * p.max_pages;
-                const int max_pages = sg.ctx < 0 ? p.max_prefix_pages : p.max_pages;
-                auto load_page = [&](int blk) -> int {
-                    const int row = blk * kBlockKeys + my_box * box_rows;
-                    if (my_box >= boxes || row >= sg.len) return 0;
-                    const int pg = table[min(row >> p.page_shift, max_pages - 1)];
-                    return min(max(pg, 0), p.num_pages - 1);
-                };
-                int page = load_page(sg.blk0);
+                since = tick();
+                int chunk = sg.blk0 * boxes / 32;
+                int entry = have_next ? entry_next_seg : load_entry(sg, chunk);
+                int entry_after = load_entry(sg, chunk + 1);
+                have_next = false;
                 // query tiles
                 if (lane == 0) {
-                    const bool single = sg.tok_end - sg.tok0 == 1;
-                    const uint32_t bytes = static_cast<uint32_t>(p.gt * (single ? 1 : p.tpt)) * G::kRowBytes;
-                    for (int u = 0; u < (sg.two ? 2 : 1) && ok; ++u) {
-                        const int slot = sg.two ? u : qs;
+                    const bool few = sg.mode == kFew;
+                    const uint32_t bytes =
+                        static_cast<uint32_t>(ln.gt * (few ? p.few_tok : ln.tpt)) * G::kRowBytes;
+                    for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
+                        const int slot = sg.mode == kTwoTiles ? u : qs;
                         if (q_cnt[slot] > 0)
-                            ok = mbar_wait(bar_qfree + slot, (q_cnt[slot] - 1) & 1, abort_flag, &g_paged_status);
+                            ok = poll(bar_qfree + slot, (q_cnt[slot] - 1) & 1);
                         if (!ok) break;
                         mbar_arrive_expect_tx(bar_q + slot, bytes);
                         for (int cb = 0; cb < G::kNumCb; ++cb)
-                            tma_load_3d(sptr + slot * G::kTileBytes + cb * G::kCbBytes,
-                                        single ? &tmQ1 : &tmQ, bar_q + slot, cb * G::kCbElems,
-                                        sg.head0, sg.tok0 + u * p.tpt);
+                            tma_load_3d(sptr + slot * G::kQSlotBytes + cb * G::kCbBytes, few ? &tmQf : &tmQ,
+                                        bar_q + slot, cb * G::kCbElems, sg.head0, sg.tok0 + u * ln.tpt);
                         ++q_cnt[slot];
                     }
                 }
-                if (!sg.two) qs ^= 1;
+                if (sg.mode != kTwoTiles) qs ^= 1;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 for (int j = 0; ok && j < sg.n_blk; ++j) {
-                    const int r0 = (sg.blk0 + j) * kBlockKeys;
+                    const int blk = sg.blk0 + j;
+                    if (blk * boxes / 32 != chunk) {
+                        ++chunk;
+                        entry = entry_after;
+                        entry_after = load_entry(sg, chunk + 1);
+                    }
+                    if (j + 1 == sg.n_blk &&
+                        __all_sync(0xffffffffu, mbar_test(seg_full + (k + 1) % kSegRing,
+                                                          ((k + 1) / kSegRing) & 1))) {
+                        const Seg nx = segs[(k + 1) % kSegRing];
+                        if (nx.n_blk > 0) {
+                            entry_next_seg = load_entry(nx, nx.blk0 * boxes / 32);
+                            have_next = true;
+                        }
+                    }
+                    const int r0 = blk * kBlockKeys;
                     const int live = min(max(sg.len - r0, 0), kBlockKeys);
                     const int nbox = (live + box_rows - 1) / box_rows;
-                    const int page_now = page;
-                    if (j + 1 < sg.n_blk) page = load_page(sg.blk0 + j + 1);
-                    const int row0 = (page_now << p.page_shift) +
-                                     ((r0 + my_box * box_rows) & ((1 << p.page_shift) - 1));
+                    // a page index outside the pool reads a wrong page instead of faulting
+                    const int page = min(max(__shfl_sync(0xffffffffu, entry, (blk * boxes + my_box) & 31), 0),
+                                         p.num_pages - 1);
+                    const int row0 = (page << ln.page_shift) +
+                                     ((r0 + my_box * box_rows) & ((1 << ln.page_shift) - 1));
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
                         const int s = kv % R;
                         if (lane == 0) {
                             if (kv >= static_cast<uint32_t>(R))
-                                ok = mbar_wait(empty + s, (kv / R - 1) & 1, abort_flag, &g_paged_status);
+                                ok = poll(empty + s, (kv / R - 1) & 1);
                             if (ok)
                                 mbar_arrive_expect_tx(full + s, static_cast<uint32_t>(nbox * box_rows) *
                                                                     G::kRowBytes);
@@ -741,86 +575,108 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // rows takes all lanes); lane 0 issues.
             constexpr uint32_t idesc_qk = make_idesc(DType<T>::kMmaFmt, 128, 128, false, false);
             constexpr uint32_t idesc_pv = make_idesc(DType<T>::kMmaFmt, 128, D, false, true);
+            constexpr uint32_t idesc_kq = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, false, false);
+            constexpr uint32_t idesc_vp = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, true, false);
+            enum { kAcc = 1, kLast = 2, kFreeV = 4, kTransposed = 8, kFreeQ = 16, kQSlot1 = 32 };
             struct Step {
                 uint32_t v;  // ring fill of its V block
                 int live;    // live keys of the block; -1: already looked after
-                int flags;   // 1: accumulate, 2: last of its stream, 4: releases V
+                int flags;
             };
             uint32_t q_cnt[2] = {0u, 0u};
             uint32_t p_cnt[2] = {0u, 0u};
             uint32_t n_s = 0, n_o = 0;  // steps issued
             uint32_t g0 = 0;            // blocks before the current segment
             int k = 0, qs = 0, cur_q = 0;
-            int i = 0, steps = 0, n_blk = 0, two = 0, len = 0, blk0 = 0;
-            bool ok = true;
-            auto next_s = [&](Step& st) -> bool {
+            int i = 0, steps = 0, n_blk = 0, mode = 0, len = 0, blk0 = 0;
+            bool q_due = false;  // the segment's query tiles are not waited for yet
+            enum { kEnd, kIssued, kStalled };
+            auto next_s = [&](Step& st) -> int {
                 if (i == steps) {
+                    const bool after_few = mode == kFew;
                     g0 += n_blk;
-                    ok = mbar_wait(seg_full + k % kSegRing, (k / kSegRing) & 1, abort_flag, &g_paged_status);
+                    ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return false;
+                    if (!ok) return kEnd;
                     const Seg& sg = segs[k % kSegRing];
                     n_blk = sg.n_blk;
-                    two = sg.two;
+                    mode = sg.mode;
                     len = sg.len;
                     blk0 = sg.blk0;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
                     ++k;
-                    if (n_blk == 0) return false;
+                    if (n_blk == 0) return kEnd;
+                    since = tick();
                     i = 0;
-                    steps = two ? 2 * n_blk : n_blk;
-                    if (two) {
-                        ok = mbar_wait(bar_q, q_cnt[0] & 1, abort_flag, &g_paged_status) &&
-                             mbar_wait(bar_q + 1, q_cnt[1] & 1, abort_flag, &g_paged_status);
+                    steps = mode == kTwoTiles ? 2 * n_blk : n_blk;
+                    q_due = true;
+                    // both query slots are needed, and the few-rows segment before
+                    // holds its own until its last product, which is not issued yet
+                    if (after_few && mode == kTwoTiles && n_s != n_o) return kStalled;
+                }
+                if (q_due) {
+                    q_due = false;
+                    if (mode == kTwoTiles) {
+                        ok = poll(bar_q, q_cnt[0] & 1) &&
+                             poll(bar_q + 1, q_cnt[1] & 1);
                         ++q_cnt[0];
                         ++q_cnt[1];
                     } else {
                         cur_q = qs;
-                        ok = mbar_wait(bar_q + qs, (qs ? q_cnt[1] : q_cnt[0]) & 1, abort_flag,
-                                       &g_paged_status);
+                        ok = poll(bar_q + qs, (qs ? q_cnt[1] : q_cnt[0]) & 1);
                         if (qs) ++q_cnt[1]; else ++q_cnt[0];
                         qs ^= 1;
                     }
                 }
+                const bool two = mode == kTwoTiles;
                 const int j = two ? i >> 1 : i;
                 const int u = two ? i & 1 : 0;
                 const uint32_t kf = 2 * (g0 + j);
                 const int s = kf % R;
                 const int t = n_s & 1;
-                if (ok && u == 0) ok = mbar_wait(full + s, (kf / R) & 1, abort_flag, &g_paged_status);
+                if (ok && u == 0) ok = poll(full + s, (kf / R) & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return false;
+                if (!ok) return kEnd;
                 const int qslot = two ? u : cur_q;
+                const bool last_in_seg = two ? j == n_blk - 1 : i == steps - 1;
                 if (lane == 0) {
                     tc_fence_after();
-                    uint64_t a0 = pg_kdesc<D>(sbase + qslot * G::kTileBytes);
+                    uint64_t a0 = pg_kdesc<D>(sbase + qslot * G::kQSlotBytes);
                     uint64_t b0 = pg_kdesc<D>(sbase + G::kOffRing + s * G::kTileBytes);
                     asm volatile("" : "+l"(a0), "+l"(b0));
+                    if (G::kHasFew && mode == kFew) {
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        mma_f16_ss(tmem + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
-                                   kk > 0 ? 1u : 0u);
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            mma_f16_ss(tmem + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
+                                       kk > 0 ? 1u : 0u);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            mma_f16_ss(tmem + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
+                                       kk > 0 ? 1u : 0u);
+                    }
                     tc_commit(bar_s + t);
                     if (!two || u == 1) tc_commit(empty + s);
-                    if (two ? j == n_blk - 1 : i == steps - 1) tc_commit(bar_qfree + qslot);
+                    if (last_in_seg && mode != kFew) tc_commit(bar_qfree + qslot);
                 }
                 __syncwarp();
                 st.v = kf + 1;
-                st.live = u == 0 ? len - (blk0 + j) * kBlockKeys : -1;
-                if (st.live < 0 && u == 0) st.live = 0;
-                st.flags = ((two ? j > 0 : i >= 2) ? 1 : 0) |
-                           ((two ? j == n_blk - 1 : i + 2 >= steps) ? 2 : 0) |
-                           ((!two || u == 1) ? 4 : 0);
+                st.live = u == 0 ? max(len - (blk0 + j) * kBlockKeys, 0) : -1;
+                st.flags = ((two ? j > 0 : i >= 2) ? kAcc : 0) |
+                           ((two ? j == n_blk - 1 : i + 2 >= steps) ? kLast : 0) |
+                           ((!two || u == 1) ? kFreeV : 0) |
+                           (mode == kFew ? kTransposed | (last_in_seg ? kFreeQ : 0) : 0) |
+                           (qslot ? kQSlot1 : 0);
                 ++i;
                 ++n_s;
-                return true;
+                return kIssued;
             };
             auto do_o = [&](const Step& st) -> bool {
                 const int t = n_o & 1;
                 const int s = st.v % R;
                 const uint32_t vbase = sbase + G::kOffRing + s * G::kTileBytes;
-                ok = mbar_wait(full + s, (st.v / R) & 1, abort_flag, &g_paged_status);
+                ok = poll(full + s, (st.v / R) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return false;
                 if (st.live >= 0 && st.live < kBlockKeys) {
@@ -828,56 +684,81 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // ring) had; zero them so that P = 0 meets no NaN
                     constexpr int kChunks = G::kSwz / 16;
                     const int n = (kBlockKeys - st.live) * kChunks;
-                    for (int e = lane; e < n * G::kNumCb; e += 32) {
-                        const int cb = e / n;
-                        const uint32_t a = vbase + cb * G::kCbBytes + st.live * G::kSwz + (e - cb * n) * 16;
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
-                    }
+#pragma unroll
+                    for (int cb = 0; cb < G::kNumCb; ++cb)
+                        for (int e = lane; e < n; e += 32) {
+                            const uint32_t a = vbase + cb * G::kCbBytes + st.live * G::kSwz + e * 16;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
+                        }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
                 uint64_t v0 = pg_vdesc<D>(vbase);
                 asm volatile("" : "+l"(v0));
+                const uint32_t o_tmem = tmem + 256 + t * 128;
                 const uint32_t par = (t ? p_cnt[1] : p_cnt[0]) & 1;
-                ok = mbar_wait(bar_p + t, par, abort_flag, &g_paged_status);
+                ok = poll(bar_p + t, par);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return false;
-                if (lane == 0) {
-                    tc_fence_after();
+                if (G::kHasFew && (st.flags & kTransposed)) {
+                    if (lane == 0) {
+                        tc_fence_after();
+                        const uint32_t q_off = (st.flags & kQSlot1) ? G::kQSlotBytes : 0;
+                        const uint64_t p0 = make_smem_desc(sbase + q_off + G::kOffPt + t * G::kPtBytes, 16, 1024,
+                                                           kLayoutSw128);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk),
-                                   idesc_pv, ((st.flags & 1) || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma_f16_ss(o_tmem, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
+                                       ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
+                    }
+                    __syncwarp();
+                } else {
+                    if (lane == 0) {
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
+                                       ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
+                    }
+                    __syncwarp();
+                    ok = poll(bar_p2 + t, par);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return false;
+                    if (lane == 0) {
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 4; kk < 8; ++kk)
+                            mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                ok = mbar_wait(bar_p2 + t, par, abort_flag, &g_paged_status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return false;
                 if (lane == 0) {
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = 4; kk < 8; ++kk)
-                        mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk),
-                                   idesc_pv, 1u);
-                    if (st.flags & 2) tc_commit(bar_o + t);
-                    if (st.flags & 4) tc_commit(empty + s);
+                    if (st.flags & kLast) tc_commit(bar_o + t);
+                    if (st.flags & kFreeV) tc_commit(empty + s);
+                    if (st.flags & kFreeQ) tc_commit(bar_qfree + ((st.flags & kQSlot1) ? 1 : 0));
                 }
                 __syncwarp();
                 if (t) ++p_cnt[1]; else ++p_cnt[0];
                 ++n_o;
                 return true;
             };
-            Step a, b, c;
-            bool more_a = next_s(a);
-            bool more_b = more_a && next_s(b);
-            while (more_a && ok) {
+            Step a, b;
+            int ahead = 0;  // steps whose S is issued and whose O is not (a, then b)
+            bool end = false;
+            while (true) {
+                while (ahead < 2 && !end) {
+                    const int got = next_s(ahead == 0 ? a : b);
+                    if (got == kStalled) break;
+                    if (got == kEnd)
+                        end = true;
+                    else
+                        ++ahead;
+                }
+                if (!ok || (ahead == 0 && end)) break;
+                if (ahead == 0) continue;
                 if (!do_o(a)) break;
-                const bool more_c = more_b && next_s(c);
-                if (!ok) break;
                 a = b;
-                more_a = more_b;
-                b = c;
-                more_b = more_c;
+                --ahead;
             }
             // all products (and their commits) retire before teardown
             if (lane == 0) {
@@ -890,24 +771,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ------------------------------------------------ units and segments
             if (lane == 0) {
                 int k = 0;
-                bool ok = true;
                 auto emit = [&](const Seg& sg) {
                     if (k >= kSegRing)
-                        ok = mbar_wait(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, abort_flag,
-                                       &g_paged_status);
+                        ok = poll(seg_free + k % kSegRing, (k / kSegRing - 1) & 1);
                     if (!ok) return;
+                    since = tick();
                     segs[k % kSegRing] = sg;
                     mbar_arrive(seg_full + k % kSegRing);
                     ++k;
                 };
-                if (x0 < x1 && *first_ctx >= c_lo) {
+                Seg sg = {};
+                if (x0 < x1 && *start_c >= c_lo) {
                     Walk w;
-                    walk_start(p, w, *first_ctx, *first_base, x0, x1, per, blockIdx.x);
-                    Seg sg;
-                    while (ok && walk_next(p, w, sg)) emit(sg);
+                    walk_start(ln, w, *start_ctx, *start_c, *start_base, x0, x1, per, blockIdx.x);
+                    while (ok && walk_next(ln, w, sg)) emit(sg);
                 }
-                Seg last = {};
-                if (ok) emit(last);
+                sg.n_blk = 0;
+                if (ok) emit(sg);
             }
             __syncwarp();
         }
@@ -917,47 +797,240 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int t = (warp - 4) >> 2;
         const int wq = warp & 3;
         const int r = wq * 32 + lane;
-        const int tok_r = r / p.gt;
-        const int head_r = r - tok_r * p.gt;
+        const int tok_r = r / ln.gt;
+        const int head_r = r - tok_r * ln.gt;
         const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
         const uint32_t s_tmem = tmem + lane_addr + t * 128;
         const uint32_t o_tmem = tmem + lane_addr + 256 + t * 128;
         const uint32_t o_other = tmem + lane_addr + 256 + (t ^ 1) * 128;
         float2* ml = reinterpret_cast<float2*>(sptr + G::kOffMl);
         const float c = p.scale_log2;
-        uint32_t s_cnt = 0, o_cnt = 0, x_cnt = 0;
-        uint32_t n0 = 0;  // steps before the segment, mod 2 matters
+        uint32_t s_cnt = 0, o_cnt = 0, x_cnt = 0, m_cnt = 0;
+        uint32_t n0 = 0;  // steps before the segment (its parity matters)
+        int qs = 0;       // query slot of the next segment of one tile
         bool y_pending = false;
-        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+            ok = __all_sync(0xffffffffu, poll(bar, parity));
+            return ok;
+        };
+        // ======================================== few rows, transposed
+        // Straight-line code for the kernel's 4, 8 or 16 columns: with one body
+        // for 16 and a test per column, instruction fetches took most of a step.
+        // Columns from ncol on hold garbage that stays in its column.
+        auto few_rows = [&](const Seg& sg, int ncol, int first, int n) {
+            const bool join = sg.n_blk > 1;
+            const bool follower = first == 1;
+            uint8_t* slot = sptr + qs * G::kQSlotBytes;
+            const uint32_t pt = sbase + qs * G::kQSlotBytes + G::kOffPt + t * G::kPtBytes +
+                                (r >> 6) * (kFewRows * 128) + (r & 7) * 2;
+            float* rmax = reinterpret_cast<float*>(slot + G::kOffMax) + t * (2 * 4 * kFewRows);
+            float* sums = reinterpret_cast<float*>(ml);  // [2 streams][4 warps][16]
+            float* maxs = sums + 2 * 4 * kFewRows;       // [16], the second stream's
+            float m_run[NC], neg_m[NC], l_part[NC];
+#pragma unroll
+            for (int g = 0; g < NC; ++g) {
+                m_run[g] = -INFINITY;
+                neg_m[g] = 0.f;
+                l_part[g] = 0.f;
+            }
+            for (int j = 0; j < n; ++j) {
+                if (!wait(bar_s + t, s_cnt & 1)) return;
+                ++s_cnt;
+                if (y_pending) {
+                    if (!wait(bar_y, (x_cnt - 1) & 1)) return;
+                    y_pending = false;
+                }
+                tc_fence_after();
+                uint32_t sv[kFewRows];
+                tmem_ld_x16(s_tmem, sv);
+                const int key0 = (sg.blk0 + first + 2 * j) * kBlockKeys;
+                if (key0 + kBlockKeys > sg.len || (ln.causal && key0 + kBlockKeys - 1 > sg.lim0)) {
+                    int lim = ln.causal ? sg.lim0 : sg.len - 1, h = 0;
+#pragma unroll
+                    for (int g = 0; g < NC; ++g) {
+                        if (key0 + r > min(lim, sg.len - 1)) sv[g] = __float_as_uint(-INFINITY);
+                        if (++h == ln.gt) {  // the next token
+                            h = 0;
+                            lim += ln.causal;
+                        }
+                    }
+                }
+                float* rm = rmax + (j & 1) * (4 * kFewRows);
+                float mx[NC];
+#pragma unroll
+                for (int g = 0; g < NC; ++g) mx[g] = warp_max(__uint_as_float(sv[g]));
+                if (lane == 0) {
+#pragma unroll
+                    for (int g = 0; g < NC; g += 4)
+                        *reinterpret_cast<float4*>(rm + wq * kFewRows + g) =
+                            make_float4(mx[g], mx[g + 1], mx[g + 2], mx[g + 3]);
+                    mbar_arrive(bar_m + t);
+                }
+                __syncwarp();
+                if (!wait(bar_m + t, m_cnt & 1)) return;
+                ++m_cnt;
+                bool grow = false;
+#pragma unroll
+                for (int g = 0; g < NC; g += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(rm + g);
+                    const float4 b = *reinterpret_cast<const float4*>(rm + kFewRows + g);
+                    const float4 d = *reinterpret_cast<const float4*>(rm + 2 * kFewRows + g);
+                    const float4 e = *reinterpret_cast<const float4*>(rm + 3 * kFewRows + g);
+                    mx[g] = fmaxf(fmax3(a.x, b.x, d.x), e.x) * c;
+                    mx[g + 1] = fmaxf(fmax3(a.y, b.y, d.y), e.y) * c;
+                    mx[g + 2] = fmaxf(fmax3(a.z, b.z, d.z), e.z) * c;
+                    mx[g + 3] = fmaxf(fmax3(a.w, b.w, d.w), e.w) * c;
+                }
+#pragma unroll
+                for (int g = 0; g < NC; ++g) grow = grow || mx[g] > m_run[g] + kRescale;
+                if (grow) {  // uniform: every thread saw the same maxima
+                    float alpha[NC];
+#pragma unroll
+                    for (int g = 0; g < NC; ++g) {
+                        alpha[g] = 1.f;
+                        if (mx[g] > m_run[g] + kRescale) {
+                            alpha[g] = ex2_approx(m_run[g] - mx[g]);
+                            m_run[g] = mx[g];
+                            neg_m[g] = -mx[g];
+                        }
+                        l_part[g] *= alpha[g];
+                    }
+                    if (j > 0) {
+                        uint32_t ov[kFewRows];
+                        tmem_ld_x16(o_tmem, ov);
+#pragma unroll
+                        for (int g = 0; g < NC; ++g)
+                            ov[g] = __float_as_uint(__uint_as_float(ov[g]) * alpha[g]);
+                        tmem_st_x16(o_tmem, ov);
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < NC; ++g) {
+                    const float pv = ex2_approx(fmaf(__uint_as_float(sv[g]), c, neg_m[g]));
+                    l_part[g] += pv;
+                    const T hv = DType<T>::from_float(pv);
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(pt + g * 128 +
+                                                                 ((((r & 63) >> 3) ^ (g & 7)) << 4)),
+                                 "h"(*reinterpret_cast<const uint16_t*>(&hv))
+                                 : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_fence_before();
+                mbar_arrive(bar_p + t);
+                mbar_arrive(bar_p2 + t);
+            }
+            if (join) ++x_cnt;
+            if (n == 0) return;
+#pragma unroll
+            for (int g = 0; g < NC; ++g) {
+                float v = l_part[g];
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+                l_part[g] = v;
+            }
+            if (!wait(bar_o + t, o_cnt & 1)) return;
+            ++o_cnt;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int g = 0; g < NC; ++g) {
+                    sums[(t * 4 + wq) * kFewRows + g] = l_part[g];
+                    if (follower && wq == 0) maxs[g] = m_run[g];
+                }
+            }
+            __syncwarp();
+            if (follower) {
+                tc_fence_before();
+                mbar_arrive(bar_x);
+                y_pending = true;
+                return;
+            }
+            if (lane == 0) mbar_arrive(bar_m + t);
+            if (!wait(bar_m + t, m_cnt & 1)) return;
+            ++m_cnt;
+            uint32_t ov[kFewRows], ov2[kFewRows];
+            tmem_ld_x16(o_tmem, ov);
+            if (join) {
+                if (!wait(bar_x, (x_cnt - 1) & 1)) return;
+                tc_fence_after();
+                tmem_ld_x16(o_other, ov2);
+            }
+            int tok = 0, h = 0;
+#pragma unroll
+            for (int g = 0; g < NC; ++g) {
+                const float* s0 = sums + t * 4 * kFewRows + g;
+                float l = (s0[0] + s0[kFewRows]) + (s0[2 * kFewRows] + s0[3 * kFewRows]);
+                float M = m_run[g], o = __uint_as_float(ov[g]);
+                if (join) {
+                    const float* s1 = sums + (t ^ 1) * 4 * kFewRows + g;
+                    const float l1 = (s1[0] + s1[kFewRows]) + (s1[2 * kFewRows] + s1[3 * kFewRows]);
+                    const float m1 = maxs[g];
+                    M = fmaxf(M, m1);
+                    const float w0 = M == -INFINITY ? 1.f : ex2_approx(m_run[g] - M);
+                    const float w1 = M == -INFINITY ? 0.f : ex2_approx(m1 - M);
+                    l = w0 * l + w1 * l1;
+                    o = w0 * o + w1 * __uint_as_float(ov2[g]);
+                }
+                o *= l > 0.f ? 1.f / l : 0.f;
+                const float lse2 = l > 0.f ? M + log2f(l) : -INFINITY;
+                if (g < ncol && h < sg.nh && r < D) {  // lane r holds column r of the head
+                    if (sg.part_row >= 0) {
+                        p.O_part[static_cast<long long>(sg.part_row) * D + ((r >> 2) * sg.part_rows + g) * 4 +
+                                 (r & 3)] = o;
+                        if (r == 0) p.L_part[sg.part_row + g] = lse2;
+                    } else {
+                        const long long orow = static_cast<long long>(sg.tok0 + tok) * ln.hq + sg.head0 + h;
+                        static_cast<T*>(p.O)[orow * D + r] = DType<T>::from_float(o);
+                        if (r == 0) p.L[orow] = lse2 * kLn2;
+                    }
+                }
+                if (++h == ln.gt) {
+                    h = 0;
+                    ++tok;
+                }
+            }
+            if (join) {
+                tc_fence_before();
+                mbar_arrive(bar_y);
+            }
+        };
         for (int k = 0; ok; ++k) {
-            ok = mbar_wait(seg_full + k % kSegRing, (k / kSegRing) & 1, abort_flag, &g_paged_status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            if (!wait(seg_full + k % kSegRing, (k / kSegRing) & 1)) break;
             const Seg sg = segs[k % kSegRing];
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
             if (sg.n_blk == 0) break;
-            const int first = (t ^ n0) & 1;  // two tiles: this stream's tile; one: its first block
-            const int tile = sg.two ? first : 0;
-            const int n = sg.two ? sg.n_blk : (sg.n_blk - first + 1) / 2;
-            n0 += sg.two ? 2 * sg.n_blk : sg.n_blk;
-            const int token = sg.tok0 + tile * p.tpt + tok_r;
-            const bool valid = tok_r < p.tpt && head_r < sg.nh && token < sg.tok_end;
+            since = tick();
+            const bool two = sg.mode == kTwoTiles;
+            const int first = (t ^ n0) & 1;  // two tiles: this stream's tile; else: its first block
+            const int n = two ? sg.n_blk : (sg.n_blk - first + 1) / 2;
+            n0 += two ? 2 * sg.n_blk : sg.n_blk;
+            const bool join = !two && sg.n_blk > 1;  // both streams have a part
+            const bool follower = !two && first == 1;
+
+            if (G::kHasFew && sg.mode == kFew) {
+                few_rows(sg, min((sg.tok_end - sg.tok0) * ln.gt, NC), first, n);
+                qs ^= 1;
+                if (!ok) break;
+                continue;
+            }
+
+            // ============================================ row tiles
+            if (!two) qs ^= 1;
+            const int tile = two ? first : 0;
+            const int token = sg.tok0 + tile * ln.tpt + tok_r;
+            const bool valid = tok_r < ln.tpt && head_r < sg.nh && token < sg.tok_end;
             const bool active = __any_sync(0xffffffffu, valid);
-            const int tile_lim = sg.lim0 + tile * p.tpt;  // first row's limit
+            const int tile_lim = sg.lim0 + tile * ln.tpt;  // first row's limit
             // last key this row sees
-            const int row_end = p.causal ? min(sg.len - 1, tile_lim + tok_r) : sg.len - 1;
+            const int row_end = ln.causal ? min(sg.len - 1, tile_lim + tok_r) : sg.len - 1;
 
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n; ++j) {
-                ok = mbar_wait(bar_s + t, s_cnt & 1, abort_flag, &g_paged_status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!wait(bar_s + t, s_cnt & 1)) break;
                 ++s_cnt;
                 if (y_pending) {  // the other stream has read the last segment's O_t
-                    ok = mbar_wait(bar_y, (x_cnt - 1) & 1, abort_flag, &g_paged_status);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!wait(bar_y, (x_cnt - 1) & 1)) break;
                     y_pending = false;
                 }
                 if (!active) {
@@ -968,9 +1041,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_after();
                 uint32_t sr[128];
                 tmem_ld_x128(s_tmem, sr);
-                const int blk = sg.blk0 + (sg.two ? j : first + 2 * j);
+                const int blk = sg.blk0 + (two ? j : first + 2 * j);
                 const int col0 = blk * kBlockKeys;
-                if (col0 + kBlockKeys > sg.len || (p.causal && col0 + kBlockKeys - 1 > tile_lim)) {
+                if (col0 + kBlockKeys > sg.len || (ln.causal && col0 + kBlockKeys - 1 > tile_lim)) {
                     const int vis = row_end - col0;  // column i is visible iff i <= vis
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
@@ -1042,29 +1115,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
 
             // ---- the segment's result
-            const bool join = !sg.two && sg.n_blk > 1;  // both streams have a part
-            if (n > 0) {
-                ok = mbar_wait(bar_o + t, o_cnt & 1, abort_flag, &g_paged_status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                ++o_cnt;
-                tc_fence_after();
-            }
             if (join) ++x_cnt;
-            if (!sg.two && first == 1) {  // second stream: hand over, or had no block
-                if (join) {
-                    ml[r] = make_float2(m_run, l_run);
-                    tc_fence_before();
-                    mbar_arrive(bar_x);
-                    y_pending = true;
-                }
+            if (n == 0) continue;
+            if (!wait(bar_o + t, o_cnt & 1)) break;
+            ++o_cnt;
+            tc_fence_after();
+            if (follower) {
+                ml[r] = make_float2(m_run, l_run);
+                tc_fence_before();
+                mbar_arrive(bar_x);
+                y_pending = true;
                 continue;
             }
-            float w0 = 1.f, w1 = 0.f;  // O = w0 O_t + w1 O_other, unnormalised sums alike
+            float w0 = 1.f, w1 = 0.f;  // O = w0 O_t + w1 O_other, and the sums alike
             if (join) {
-                ok = mbar_wait(bar_x, (x_cnt - 1) & 1, abort_flag, &g_paged_status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!wait(bar_x, (x_cnt - 1) & 1)) break;
                 tc_fence_after();
                 const float2 o2 = ml[r];
                 const float M = fmaxf(m_run, o2.x);
@@ -1079,10 +1144,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             w0 *= inv_l;
             w1 *= inv_l;
             const float lse2 = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
-            const int head = sg.head0 + head_r;
             if (active) {
-                const long long prow = static_cast<long long>(sg.part_row) + tile * kTileRows + r;
-                const long long orow = static_cast<long long>(token) * p.hq + head;
+                const long long prow = static_cast<long long>(sg.part_row) + tile * kTileRows;
+                const long long orow = static_cast<long long>(token) * ln.hq + sg.head0 + head_r;
 #pragma unroll
                 for (int cb = 0; cb < D / 32; ++cb) {
                     uint32_t o[32];
@@ -1098,11 +1162,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     if (valid) {
                         if (sg.part_row >= 0) {
-                            float4* dst = reinterpret_cast<float4*>(p.O_part + prow * D + cb * 32);
+                            float4* dst = reinterpret_cast<float4*>(p.O_part + prow * D) + r;
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                                dst[(cb * 8 + i) * sg.part_rows] =
+                                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
                         } else {
                             uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + orow * D + cb * 32);
 #pragma unroll
@@ -1119,7 +1184,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 if (valid) {
                     if (sg.part_row >= 0)
-                        p.L_part[prow] = lse2;
+                        p.L_part[prow + r] = lse2;
                     else
                         p.L[orow] = lse2 * kLn2;
                 }
@@ -1131,6 +1196,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
 
+    if (!ok && lane == 0 && !*abort_flag) {
+        *abort_flag = 1;
+        record_status(&g_paged_status, kStatusWaitTimeout);
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -1139,40 +1208,74 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
-// Joins normalised partial rows by their log2-sum-exp: one warp per row, a
-// lane holds D/32 columns.  `row_of(k)` is the k-th partial's row.
-template <typename T, int D, typename RowOf>
-__device__ __forceinline__ void join_rows(const TcParams& p, int n, RowOf row_of, long long out_row) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
-    float M = -INFINITY;
-    for (int k = lane; k < n; k += 32) M = fmaxf(M, p.L_part[row_of(k)]);
+// ---------------------------------------------------------------------------
+// The second kernel: joins partial rows by their log2-sum-exp, in the order of
+// the line.  A block takes 32 rows (one per lane, so that loads of the
+// partials' layout are contiguous); its 8 warps share the columns, four at a
+// time, and the result is transposed through shared memory for its stores.
+// Bound by latency (two dependent rounds of loads), not bytes.
+// ---------------------------------------------------------------------------
+constexpr int kJoinThreads = 256;
+
+template <int D>
+struct JoinAcc {
+    static constexpr int kQuads = D / 4 / (kJoinThreads / 32);  // per warp
+    float4 v[kQuads];
+    float tot;
+};
+
+template <int D>
+__device__ __forceinline__ void join_add(const TcParams& p, JoinAcc<D>& a, float M, int base, int rows,
+                                         int r) {
+    const float w = sm100::ex2_approx(p.L_part[base + r] - M);
+    a.tot += w;
+    const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(base) * D) + r +
+                        (threadIdx.x >> 5) * JoinAcc<D>::kQuads * rows;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    float acc[V], tot = 0.f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    if (M != -INFINITY) {
-        for (int k0 = 0; k0 < n; k0 += 32) {
-            const float w = k0 + lane < n ? sm100::ex2_approx(p.L_part[row_of(k0 + lane)] - M) : 0.f;
-            tot += w;
-            const int m = min(32, n - k0);
-#pragma unroll 4
-            for (int k = 0; k < m; ++k) {
-                const float wk = __shfl_sync(0xffffffffu, w, k);
-                const float* src = p.O_part + row_of(k0 + k) * D + lane * V;
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] = fmaf(wk, src[e], acc[e]);
-            }
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, off);
+    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) {
+        const float4 s = src[q * rows];
+        a.v[q].x = fmaf(w, s.x, a.v[q].x);
+        a.v[q].y = fmaf(w, s.y, a.v[q].y);
+        a.v[q].z = fmaf(w, s.z, a.v[q].z);
+        a.v[q].w = fmaf(w, s.w, a.v[q].w);
     }
-    const float inv = tot > 0.f ? 1.f / tot : 0.f;
-    T* dst = static_cast<T*>(p.O) + out_row * D + lane * V;
+}
+
+// Writes this block's 32 rows; lane's row goes to out_row (-1: none).
+template <typename T, int D>
+__device__ __forceinline__ void join_store(const TcParams& p, const JoinAcc<D>& a, float M, int out_row) {
+    constexpr int kPitch = D + 8;  // 16-bit elements; rows 16 bytes apart in the banks
+    __shared__ __align__(16) T tile[32][kPitch];
+    __shared__ int rows[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float inv = a.tot > 0.f ? 1.f / a.tot : 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) dst[e] = DType<T>::from_float(acc[e] * inv);
-    if (lane == 0) p.L[out_row] = tot > 0.f ? (M + log2f(tot)) * kLn2 : -INFINITY;
+    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) {
+        uint2 v;
+        v.x = DType<T>::pack2(a.v[q].x * inv, a.v[q].y * inv);
+        v.y = DType<T>::pack2(a.v[q].z * inv, a.v[q].w * inv);
+        *reinterpret_cast<uint2*>(&tile[lane][(warp * JoinAcc<D>::kQuads + q) * 4]) = v;
+    }
+    if (warp == 0) {
+        rows[lane] = out_row;
+        if (out_row >= 0) p.L[out_row] = a.tot > 0.f ? (M + log2f(a.tot)) * kLn2 : -INFINITY;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * (D / 8); e += kJoinThreads) {
+        const int r = e / (D / 8), c = e - r * (D / 8);
+        if (rows[r] >= 0)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(rows[r]) * D + c * 8) =
+                *reinterpret_cast<const uint4*>(&tile[r][c * 8]);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ JoinAcc<D> join_zero() {
+    JoinAcc<D> a;
+#pragma unroll
+    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) a.v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    a.tot = 0.f;
+    return a;
 }
 
 __device__ __forceinline__ bool partials_ready() {
@@ -1181,133 +1284,128 @@ __device__ __forceinline__ bool partials_ready() {
     return *reinterpret_cast<const volatile int*>(&g_paged_status.code) == 0;
 }
 
-// One warp per (sequence, query head): the prefix's partials, then its own.
+// Block (head chunk, 32 rows of the batch's row tiles): the prefix's partials,
+// then the sequence's own.
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
-    paged_join_prefix_kernel(const TcParams p) {
-    const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= static_cast<long long>(p.B) * p.hq) return;
-    const int b = static_cast<int>(row / p.hq);
-    const int h = static_cast<int>(row - static_cast<long long>(b) * p.hq);
-    const Ctx pre = load_ctx(p, -1), own = load_ctx(p, b);
+__global__ void __launch_bounds__(kJoinThreads)
+    paged_join_prefix_kernel(const __grid_constant__ TcParams p, int groups) {
+    const PagedLine& ln = p.ln;
+    const int hc = blockIdx.x / groups;
+    const int row = (blockIdx.x - hc * groups) * 32 + (threadIdx.x & 31);  // of the head chunk
+    const int tile = row / kTileRows;
+    const int r = row - tile * kTileRows;
+    const int tok_r = r / ln.gt;
+    const int hr = r - tok_r * ln.gt;
+    const int b = tile * ln.tpt + tok_r;
+    const int hk = hc / ln.chunks, ch = hc - hk * ln.chunks;
+    const bool valid = tok_r < ln.tpt && b < ln.B && ch * ln.gt + hr < ln.group;
+    const Ctx pre = load_ctx(ln, -1);
+    const Ctx own = load_ctx(ln, valid ? b : 0);
     if (!partials_ready()) return;
-    const PrefixParts q = prefix_parts(p, pre, own, b, h);
-    join_rows<T, D>(
-        p, q.n1 + q.n2,
-        [&](int k) -> long long {
-            return k < q.n1 ? q.row1 + static_cast<long long>(k) * (2 * kTileRows)
-                            : q.row2 + static_cast<long long>(k - q.n1) * p.gt;
-        },
-        row);
+    PrefixParts q = {};
+    if (valid) q = prefix_parts(ln, *ln.per, pre, own, b, hc, hr);
+    float M = -INFINITY;
+    for (int k = 0; k < q.n1; ++k) M = fmaxf(M, p.L_part[q.row1 + k * (2 * kTileRows) + q.r1]);
+    for (int k = 0; k < q.n2; ++k) M = fmaxf(M, p.L_part[q.row2 + k * ln.gt + q.r2]);
+    JoinAcc<D> a = join_zero<D>();
+    if (M != -INFINITY) {
+#pragma unroll 2
+        for (int k = 0; k < q.n1; ++k) join_add<D>(p, a, M, q.row1 + k * (2 * kTileRows), kTileRows, q.r1);
+        for (int k = 0; k < q.n2; ++k) join_add<D>(p, a, M, q.row2 + k * ln.gt, ln.gt, q.r2);
+    }
+    join_store<T, D>(p, a, M, valid ? b * ln.hq + hk * ln.group + ch * ln.gt + hr : -1);
 }
 
 // Block (i, y): rows [32 y, 32 y + 32) of the unit whose first blocks CTA i
 // had and whose last CTA split[i].last had.
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    paged_join_split_kernel(const TcParams p) {
+__global__ void __launch_bounds__(kJoinThreads)
+    paged_join_split_kernel(const __grid_constant__ TcParams p, int) {
+    const PagedLine& ln = p.ln;
     if (!partials_ready()) return;
-    const Split sp = p.split[blockIdx.x];
     const int i = static_cast<int>(blockIdx.x);
+    const Split sp = ln.split[i];
     if (sp.last <= i) return;
-    for (int q = 0; q < 4; ++q) {
-        const int rr = blockIdx.y * 32 + (threadIdx.x >> 5) * 4 + q;
-        const int tile = rr / kTileRows;
-        const int r = rr - tile * kTileRows;
-        const int tok_r = r / p.gt;
-        const int head_r = r - tok_r * p.gt;
-        const int token = sp.tok0 + tile * p.tpt + tok_r;
-        if ((tile == 1 && !sp.two) || tok_r >= p.tpt || head_r >= sp.nh || token >= sp.tok_end) continue;
-        join_rows<T, D>(
-            p, sp.last - i + 1,
-            [&](int k) -> long long {
-                return static_cast<long long>(2 * (i + k) + (k == 0 ? 1 : 0)) * (2 * kTileRows) + rr;
-            },
-            static_cast<long long>(token) * p.hq + sp.head0 + head_r);
+    const int row = blockIdx.y * 32 + (threadIdx.x & 31);
+    const int tile = row / kTileRows;
+    const int r = row - tile * kTileRows;
+    if (tile == 1 && sp.mode != kTwoTiles) return;
+    const int tok_r = r / ln.gt;
+    const int hr = r - tok_r * ln.gt;
+    const int token = sp.tok0 + tile * ln.tpt + tok_r;
+    const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
+    if (__syncthreads_or(valid) == 0) return;
+    const int n = valid ? sp.last - i + 1 : 0;
+    auto base = [&](int k) { return (2 * (i + k) + (k == 0 ? 1 : 0)) * (2 * kTileRows) + tile * kTileRows; };
+    float M = -INFINITY;
+    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[base(k) + r]);
+    JoinAcc<D> a = join_zero<D>();
+    if (M != -INFINITY) {
+#pragma unroll 2
+        for (int k = 0; k < n; ++k) join_add<D>(p, a, M, base(k), kTileRows, r);
     }
+    join_store<T, D>(p, a, M, valid ? token * ln.hq + sp.head0 + hr : -1);
 }
 
 // Launches `kern` so that its blocks may be scheduled while the kernel before
 // it on the stream still runs (they wait for it inside).
-template <typename... Args>
-cudaError_t launch_behind(void (*kern)(Args...), dim3 grid, int threads, cudaStream_t stream,
-                          const TcParams& p) {
+cudaError_t launch_behind(void (*kern)(const TcParams, int), dim3 grid, cudaStream_t stream,
+                          const TcParams& p, int arg) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p);
+    return cudaLaunchKernelEx(&cfg, kern, p, arg);
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-// Row tiles of the query heads and tokens, and the line's scale.
-void set_tiles(TcParams& p) {
-    p.group = p.hq / p.hkv;
-    p.chunks = (p.group + kTileRows - 1) / kTileRows;
-    p.gt = (p.group + p.chunks - 1) / p.chunks;
-    p.tpt = kTileRows / p.gt;
-    p.w_two = 2;
-    p.w_one = 1;
-    p.min_per = 2;  // at least the larger weight: every CTA of a unit has a block of it
-}
-
-// Partial rows and record bytes of a launch of `grid` CTAs.  Going along the
-// line, each piece starts a new unit, a new CTA or both, so unit + CTA numbers
-// the pieces; in ragged mode only a CTA's first and last piece are partial.
-void set_parts(TcParams& p, int grid, long long& rows, long long& records) {
-    const long long heads = static_cast<long long>(p.hkv) * p.chunks;
-    if (p.prefix_mode) {
-        const long long tiles = (p.B + p.tpt - 1) / p.tpt;
-        p.own_part_row = (heads * ((tiles + 1) / 2) + grid) * 2 * kTileRows;
-        rows = p.own_part_row + (heads * p.B + grid) * p.gt;
-        records = heads * p.B * static_cast<long long>(sizeof(long long));
-    } else {
-        rows = 2LL * grid * 2 * kTileRows;
-        records = grid * static_cast<long long>(sizeof(Split));
-    }
-}
-
-template <typename T, int D>
+template <typename T, int D, int NC>
 FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     using G = PagedGeom<D>;
     TcParams p{};
+    PagedLine& ln = p.ln;
     p.O = a.O;
     p.L = a.L;
     p.prefix_table = a.prefix_table;
-    p.prefix_len = a.prefix_len;
     p.block_table = a.block_table;
-    p.seq_lens = a.seq_lens;
-    p.cu_seqlens = a.cu_seqlens;
-    p.prefix_mode = a.prefix_table != nullptr;
-    p.num_tokens = a.num_tokens;
-    p.B = a.B;
-    p.hq = a.hq;
-    p.hkv = a.hkv;
-    set_tiles(p);
-    p.page_shift = a.page_shift;
-    p.max_prefix_pages = a.max_prefix_pages;
-    p.max_pages = a.max_pages;
     p.num_pages = a.num_pages;
-    p.causal = a.causal;
     // a zero scale becomes a tiny positive one so that masked scores stay -inf
     p.scale_log2 = fmaxf(a.scale_log2, 1e-30f);
+    ln.prefix_len = a.prefix_len;
+    ln.seq_lens = a.seq_lens;
+    ln.cu_seqlens = a.cu_seqlens;
+    ln.prefix_mode = a.prefix_table != nullptr;
+    ln.causal = a.causal;
+    ln.num_tokens = a.num_tokens;
+    ln.B = a.B;
+    ln.hq = a.hq;
+    ln.hkv = a.hkv;
+    ln.page_shift = a.page_shift;
+    ln.max_prefix_pages = a.max_prefix_pages;
+    ln.max_pages = a.max_pages;
+    set_tiles(ln, G::kHasFew ? NC : 0);
+    p.few_tok = std::max(1, kFewRows / ln.gt);
+    const int grid = persistent_grid(0x7fffffffLL, 1);
+    long long rows, records;
+    if (!set_parts(ln, grid, rows, records)) return FlashAttentionError::INVALID_DIMENSION;
 
     const CUtensorMapDataType dt = DType<T>::kTmaType;
     const CUtensorMapSwizzle swz = G::kSwz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    CUtensorMap mq, mq1, mk, mv;
+    CUtensorMap mq, mqf, mk, mv;
     {
         const uint64_t dims[3] = {D, static_cast<uint64_t>(a.hq), static_cast<uint64_t>(a.num_tokens)};
         const uint64_t strides[2] = {D * 2, static_cast<uint64_t>(a.hq) * D * 2};
-        const uint32_t box[3] = {G::kCbElems, static_cast<uint32_t>(p.gt), static_cast<uint32_t>(p.tpt)};
-        const uint32_t box1[3] = {G::kCbElems, static_cast<uint32_t>(p.gt), 1};
+        const uint32_t gt = static_cast<uint32_t>(ln.gt);
+        const uint32_t box[3] = {G::kCbElems, gt, static_cast<uint32_t>(ln.tpt)};
+        const uint32_t boxf[3] = {G::kCbElems, gt, static_cast<uint32_t>(p.few_tok)};
         if (!encode_tmap_3d_strided(&mq, a.Q, dt, dims, strides, box, swz) ||
-            !encode_tmap_3d_strided(&mq1, a.Q, dt, dims, strides, box1, swz))
+            !encode_tmap_3d_strided(&mqf, a.Q, dt, dims, strides, boxf, swz))
             return FlashAttentionError::CUDA_ERROR;
     }
     {
@@ -1320,15 +1418,11 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
             !encode_tmap_3d_strided(&mv, a.V, dt, dims, strides, box, swz))
             return FlashAttentionError::CUDA_ERROR;
     }
-    auto kern = paged_attn_kernel<T, D>;
+    auto kern = paged_attn_kernel<T, D, NC>;
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), G::kSmemBytes))
         return FlashAttentionError::CUDA_ERROR;
-    const int grid = persistent_grid(0x7fffffffLL, 1);
 
-    // workspace: line scale, unit starts or split records, partial rows
-    long long rows, records;
-    set_parts(p, grid, rows, records);
-    if (rows > 0x7fffffffLL) return FlashAttentionError::INVALID_DIMENSION;
+    // workspace: piece length, unit starts or split records, partial rows
     const size_t off_rec = 256;
     const size_t off_l = off_rec + align256(static_cast<size_t>(records));
     const size_t off_o = off_l + align256(static_cast<size_t>(rows) * sizeof(float));
@@ -1337,22 +1431,25 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     const FlashAttentionError werr = workspace_alloc(&ws, bytes, stream);
     if (werr != FlashAttentionError::SUCCESS) return werr;
     char* base = static_cast<char*>(ws);
-    p.per = reinterpret_cast<long long*>(base);
-    p.unit_start = reinterpret_cast<long long*>(base + off_rec);
-    p.split = reinterpret_cast<Split*>(base + off_rec);
+    ln.per = reinterpret_cast<int*>(base);
+    ln.unit_start = reinterpret_cast<int*>(base + off_rec);
+    ln.split = reinterpret_cast<Split*>(base + off_rec);
     p.L_part = reinterpret_cast<float*>(base + off_l);
     p.O_part = reinterpret_cast<float*>(base + off_o);
 
     bind_status_word(reinterpret_cast<const void*>(&g_paged_status), stream);
-    kern<<<grid, kTcThreads, G::kSmemBytes, stream>>>(mq, mq1, mk, mv, p);
+    kern<<<grid, kTcThreads, G::kSmemBytes, stream>>>(mq, mqf, mk, mv, p);
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) {
-        if (p.prefix_mode)
+        if (ln.prefix_mode) {
+            const long long tiles = (ln.B + ln.tpt - 1) / ln.tpt;
+            const long long last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
+            const int groups = static_cast<int>((tiles - 1) * (kTileRows / 32) + (last + 31) / 32);
             err = launch_behind(paged_join_prefix_kernel<T, D>,
-                                dim3(static_cast<unsigned>((static_cast<long long>(p.B) * p.hq + 3) / 4)),
-                                128, stream, p);
-        else
-            err = launch_behind(paged_join_split_kernel<T, D>, dim3(grid, 8), 256, stream, p);
+                                dim3(static_cast<unsigned>(ln.hkv * ln.chunks * groups)), stream, p, groups);
+        } else {
+            err = launch_behind(paged_join_split_kernel<T, D>, dim3(grid, 2 * kTileRows / 32), stream, p, 0);
+        }
         if (err != cudaSuccess) cudaGetLastError();
     }
     workspace_free(ws, stream);
@@ -1361,7 +1458,14 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
 
 template <typename T, int D>
 FlashAttentionError paged_typed(const PagedParams<T>& p, cudaStream_t stream) {
-    return p.page_shift >= 3 ? paged_tc<T, D>(p, stream) : paged_row<T, D>(p, stream);
+    if (p.page_shift < 3) return paged_row<T, D>(p, stream);
+    if constexpr (PagedGeom<D>::kHasFew) {
+        // one token's heads fit the few-rows form up to groups of 16
+        const int group = p.hq / p.hkv;
+        if (group > 4 && group <= 8) return paged_tc<T, D, 8>(p, stream);
+        if (group > 8 && group <= 16) return paged_tc<T, D, 16>(p, stream);
+    }
+    return paged_tc<T, D, 4>(p, stream);
 }
 
 }  // namespace

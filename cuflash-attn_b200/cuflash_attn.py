@@ -138,11 +138,11 @@ class CuFlashError(RuntimeError):
         self.code = code
 
 
-_SUFFIX = {"float32": "f32", "float16": "f16", "bfloat16": "bf16"}
+_SUFFIX = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
 
 
 def _suffix(t) -> str:
-    name = str(t.dtype).replace("torch.", "")
+    name = str(t.dtype)
     if name not in _SUFFIX:
         raise CuFlashError(UNSUPPORTED_DTYPE, f"Unsupported data type {t.dtype}")
     return _SUFFIX[name]
@@ -179,50 +179,51 @@ def rope_table(max_position: int, rotary_dim: int, base: float = 10000.0, device
 
 
 def _token_stride(t) -> int:
-    """Elements between tokens of t [tokens, heads, D] whose heads are packed."""
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    """Elements between tokens of t [tokens, heads, D] whose heads are packed
+    (0 where there is only one)."""
+    tokens, heads, D = t.shape
+    between, head, element = t.stride()
+    if element != 1 or (heads > 1 and head != D):
         raise ValueError("a token's heads must be contiguous")
-    if t.shape[0] <= 1:
+    if tokens <= 1:
         return 0
-    if t.stride(0) < t.shape[1] * t.shape[2]:
+    if between < heads * D:
         raise ValueError("tokens must not overlap")
-    return t.stride(0)
+    return between
 
 
-def _check_like(ref, **tensors) -> None:
-    """Same device and dtype as ref."""
+# The checks of the paged-cache entries, which run once per token of a serving
+# loop: device numbers, dtypes and sizes are compared with as few calls into
+# torch as there are tensors, and what is wrong is only worked out for the error.
+def _check_packed(dtype, **tensors) -> None:
+    """Contiguous tensors of one type."""
     for name, t in tensors.items():
-        if t.device != ref.device:
-            raise ValueError(f"{name} must be on {ref.device}")
-        if t.dtype != ref.dtype:
-            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {ref.dtype}")
+        if t.dtype is not dtype:
+            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {dtype}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
 
 
-def _check_lse(ref, L) -> None:
+def _check_device(device: int, *tensors) -> None:
+    """All on CUDA device `device` (-1: the first one is on none)."""
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"every tensor must be on one CUDA device, not {t.device}")
+
+
+def _mismatch(name, t, shape):
+    return CuFlashError(DIMENSION_MISMATCH, f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
+
+
+def _run_on(device: int, stream, call):
+    """call(raw stream) with `device` current; by default on its current stream."""
     import torch
 
-    if L.dtype != torch.float32 or L.device != ref.device:
-        raise ValueError(f"L must be float32 on {ref.device}")
-
-
-def _check_index(ref, **tensors) -> None:
-    """int32 tensors on ref's device."""
-    import torch
-
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.device != ref.device:
-            raise ValueError(f"{name} must be on {ref.device}")
-        if t.dtype != torch.int32:
-            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be int32")
-
-
-def _check_shape(**pairs) -> None:
-    for name, (t, shape) in pairs.items():
-        if tuple(t.shape) != tuple(shape):
-            raise CuFlashError(DIMENSION_MISMATCH,
-                               f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
+    raw = (torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+    if torch._C._cuda_getDevice() == device:
+        return call(raw)
+    with torch.cuda.device(device):
+        return call(raw)
 
 
 class CuFlashAttn:
@@ -356,43 +357,66 @@ class CuFlashAttn:
         one projection's output.  Returns Q_out (None without Q)."""
         import torch
 
-        tokens, Hkv, D = K.shape
-        num_pages, page_size = K_cache.shape[:2]
+        tokens, Hkv, D = shape = K.shape
+        num_pages, page_size, cache_heads, cache_dim = K_cache.shape
         B, max_pages = block_table.shape
-        Hq = 0 if Q is None else Q.shape[1]
-        _check_shape(V=(V, K.shape), K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
-                     V_cache=(V_cache, K_cache.shape), seq_lens=(seq_lens, (B,)))
-        _check_like(K, V=V, K_cache=K_cache, V_cache=V_cache)
-        _check_index(K, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
-                     positions=positions)
+        dtype, device = K.dtype, K.get_device()
+        if V.shape != shape:
+            raise _mismatch("V", V, shape)
+        if cache_heads != Hkv or cache_dim != D:
+            raise _mismatch("K_cache", K_cache, (num_pages, page_size, Hkv, D))
+        if V_cache.shape != K_cache.shape:
+            raise _mismatch("V_cache", V_cache, K_cache.shape)
+        if seq_lens.shape != (B,):
+            raise _mismatch("seq_lens", seq_lens, (B,))
+        if V.dtype is not dtype:
+            raise CuFlashError(UNSUPPORTED_DTYPE, f"V must be {dtype}, not {V.dtype}")
+        _check_packed(dtype, K_cache=K_cache, V_cache=V_cache)
+        _check_packed(torch.int32, block_table=block_table, seq_lens=seq_lens)
+        k_stride, v_stride, q_stride = _token_stride(K), _token_stride(V), 0
+        Hq = q_ptr = out_ptr = cu_ptr = pos_ptr = rope_ptr = max_position = rotary = 0
         if cu_seqlens is not None:
-            _check_shape(cu_seqlens=(cu_seqlens, (B + 1,)))
+            if cu_seqlens.shape != (B + 1,):
+                raise _mismatch("cu_seqlens", cu_seqlens, (B + 1,))
+            _check_packed(torch.int32, cu_seqlens=cu_seqlens)
+            _check_device(device, cu_seqlens)
+            cu_ptr = cu_seqlens.data_ptr()
         if positions is not None:
-            _check_shape(positions=(positions, (tokens,)))
+            if positions.shape != (tokens,):
+                raise _mismatch("positions", positions, (tokens,))
+            _check_packed(torch.int32, positions=positions)
+            _check_device(device, positions)
+            pos_ptr = positions.data_ptr()
         if Q is not None:
-            _check_shape(Q=(Q, (tokens, Hq, D)))
+            Hq = Q.shape[1]
+            if Q.shape != (tokens, Hq, D):
+                raise _mismatch("Q", Q, (tokens, Hq, D))
+            if Q.dtype is not dtype:
+                raise CuFlashError(UNSUPPORTED_DTYPE, f"Q must be {dtype}, not {Q.dtype}")
+            q_stride = _token_stride(Q)
             if Q_out is None:
-                Q_out = torch.empty((tokens, Hq, D), device=Q.device, dtype=Q.dtype)
-            _check_shape(Q_out=(Q_out, Q.shape))
-            _check_like(K, Q=Q, Q_out=Q_out)
+                Q_out = torch.empty((tokens, Hq, D), device=Q.device, dtype=dtype)
+            elif Q_out.shape != Q.shape:
+                raise _mismatch("Q_out", Q_out, Q.shape)
+            _check_packed(dtype, Q_out=Q_out)
+            _check_device(device, Q, Q_out)
+            q_ptr, out_ptr = Q.data_ptr(), Q_out.data_ptr()
         elif Q_out is not None:
             raise ValueError("Q_out without Q")
-        max_position = rotary = 0
         if rope_table is not None:
-            if rope_table.dtype != torch.float32 or rope_table.device != K.device:
-                raise ValueError(f"rope_table must be float32 on {K.device}")
+            _check_packed(torch.float32, rope_table=rope_table)
+            _check_device(device, rope_table)
             max_position, rotary = rope_table.shape
-        strides = [0 if t is None else _token_stride(t) for t in (Q, K, V)]
-        data = [ctypes.c_void_p(0 if t is None else t.data_ptr()) for t in (Q, K, V)]
-        if not K.is_cuda:
-            raise ValueError("tensor must be on a CUDA device")
-        fn = getattr(self.lib, f"cuflash_kv_append_paged_{_suffix(K)}")
-        with torch.cuda.device(K.device):
-            self.check_error(fn(*data, _ptr(Q_out), _ptr(K_cache), _ptr(V_cache),
-                                _ptr(rope_table), _ptr(positions), _ptr(block_table),
-                                _ptr(seq_lens), _ptr(cu_seqlens), tokens, B, Hq, Hkv, D,
-                                page_size, max_pages, num_pages, *strides, rotary, max_position,
-                                bool(interleaved), _stream_handle(stream)))
+            rope_ptr = rope_table.data_ptr()
+        _check_device(device, K, V, K_cache, V_cache, block_table, seq_lens)
+        fn = getattr(self.lib, "cuflash_kv_append_paged_" + _suffix(K))
+        code = _run_on(device, stream, lambda raw: fn(
+            q_ptr, K.data_ptr(), V.data_ptr(), out_ptr, K_cache.data_ptr(), V_cache.data_ptr(),
+            rope_ptr, pos_ptr, block_table.data_ptr(), seq_lens.data_ptr(), cu_ptr, tokens, B, Hq,
+            Hkv, D, page_size, max_pages, num_pages, q_stride, k_stride, v_stride, rotary,
+            max_position, interleaved, raw))
+        if code:
+            self.check_error(code)
         return Q_out
 
     def forward_paged(self, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens,
@@ -403,25 +427,31 @@ class CuFlashAttn:
         bottom-right.  Returns O [tokens, Hq, D], L [tokens, Hq]."""
         import torch
 
-        tokens, Hq, D = Q.shape
-        num_pages, page_size, Hkv, _ = K_cache.shape
+        tokens, Hq, D = shape = Q.shape
+        num_pages, page_size, Hkv, cache_dim = K_cache.shape
         B, max_pages = block_table.shape
-        if scale is None:
-            scale = 1.0 / math.sqrt(D)
-        O = torch.empty_like(Q) if O is None else O
-        L = torch.empty((tokens, Hq), device=Q.device, dtype=torch.float32) if L is None else L
-        _check_shape(K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
-                     V_cache=(V_cache, K_cache.shape), seq_lens=(seq_lens, (B,)),
-                     cu_seqlens=(cu_seqlens, (B + 1,)), O=(O, Q.shape), L=(L, (tokens, Hq)))
-        _check_like(Q, K_cache=K_cache, V_cache=V_cache, O=O)
-        _check_lse(Q, L)
-        _check_index(Q, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens)
-        fn = getattr(self.lib, f"cuflash_attention_forward_paged_{_suffix(Q)}")
-        with torch.cuda.device(Q.device):
-            self.check_error(fn(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_table),
-                                _ptr(seq_lens), _ptr(cu_seqlens), _ptr(O), _ptr(L), tokens, B,
-                                Hq, Hkv, D, page_size, max_pages, num_pages, float(scale),
-                                bool(causal), _stream_handle(stream)))
+        dtype, device = Q.dtype, Q.get_device()
+        if cache_dim != D:
+            raise _mismatch("K_cache", K_cache, (num_pages, page_size, Hkv, D))
+        if V_cache.shape != K_cache.shape:
+            raise _mismatch("V_cache", V_cache, K_cache.shape)
+        if seq_lens.shape != (B,):
+            raise _mismatch("seq_lens", seq_lens, (B,))
+        if cu_seqlens.shape != (B + 1,):
+            raise _mismatch("cu_seqlens", cu_seqlens, (B + 1,))
+        _check_packed(dtype, Q=Q, K_cache=K_cache, V_cache=V_cache)
+        _check_packed(torch.int32, block_table=block_table, seq_lens=seq_lens,
+                      cu_seqlens=cu_seqlens)
+        _check_device(device, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens)
+        O, L = self._outputs(Q, shape, (tokens, Hq), O, L)
+        fn = getattr(self.lib, "cuflash_attention_forward_paged_" + _suffix(Q))
+        code = _run_on(device, stream, lambda raw: fn(
+            Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), block_table.data_ptr(),
+            seq_lens.data_ptr(), cu_seqlens.data_ptr(), O.data_ptr(), L.data_ptr(), tokens, B, Hq,
+            Hkv, D, page_size, max_pages, num_pages,
+            D ** -0.5 if scale is None else scale, causal, raw))
+        if code:
+            self.check_error(code)
         return O, L
 
     def decode_shared_prefix(self, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
@@ -433,28 +463,59 @@ class CuFlashAttn:
         L [B, Hq]."""
         import torch
 
-        B, Hq, _, D = q.shape
-        num_pages, page_size, Hkv, _ = K_cache.shape
-        max_pages = block_table.shape[1]
-        if scale is None:
-            scale = 1.0 / math.sqrt(D)
-        O = torch.empty_like(q) if O is None else O
-        L = torch.empty((B, Hq), device=q.device, dtype=torch.float32) if L is None else L
-        _check_shape(q=(q, (B, Hq, 1, D)), K_cache=(K_cache, (num_pages, page_size, Hkv, D)),
-                     V_cache=(V_cache, K_cache.shape), prefix_len=(prefix_len, (1,)),
-                     prefix_table=(prefix_table, (prefix_table.numel(),)),
-                     block_table=(block_table, (B, max_pages)), seq_lens=(seq_lens, (B,)),
-                     O=(O, q.shape), L=(L, (B, Hq)))
-        _check_like(q, K_cache=K_cache, V_cache=V_cache, O=O)
-        _check_lse(q, L)
-        _check_index(q, prefix_table=prefix_table, prefix_len=prefix_len,
-                     block_table=block_table, seq_lens=seq_lens)
-        fn = getattr(self.lib, f"cuflash_attention_decode_shared_prefix_{_suffix(q)}")
-        with torch.cuda.device(q.device):
-            self.check_error(fn(_ptr(q), _ptr(K_cache), _ptr(V_cache), _ptr(prefix_table),
-                                _ptr(prefix_len), _ptr(block_table), _ptr(seq_lens), _ptr(O),
-                                _ptr(L), B, Hq, Hkv, D, page_size, prefix_table.numel(),
-                                max_pages, num_pages, float(scale), _stream_handle(stream)))
+        B, Hq, one, D = shape = q.shape
+        num_pages, page_size, Hkv, cache_dim = K_cache.shape
+        rows, max_pages = block_table.shape
+        (max_prefix,) = prefix_table.shape
+        dtype, device = q.dtype, q.get_device()
+        if one != 1:
+            raise _mismatch("q", q, (B, Hq, 1, D))
+        if cache_dim != D:
+            raise _mismatch("K_cache", K_cache, (num_pages, page_size, Hkv, D))
+        if V_cache.shape != K_cache.shape:
+            raise _mismatch("V_cache", V_cache, K_cache.shape)
+        if rows != B:
+            raise _mismatch("block_table", block_table, (B, max_pages))
+        if seq_lens.shape != (B,):
+            raise _mismatch("seq_lens", seq_lens, (B,))
+        if prefix_len.shape != (1,):
+            raise _mismatch("prefix_len", prefix_len, (1,))
+        _check_packed(dtype, q=q, K_cache=K_cache, V_cache=V_cache)
+        _check_packed(torch.int32, prefix_table=prefix_table, prefix_len=prefix_len,
+                      block_table=block_table, seq_lens=seq_lens)
+        _check_device(device, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
+                      seq_lens)
+        O, L = self._outputs(q, shape, (B, Hq), O, L)
+        fn = getattr(self.lib, "cuflash_attention_decode_shared_prefix_" + _suffix(q))
+        code = _run_on(device, stream, lambda raw: fn(
+            q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_table.data_ptr(),
+            prefix_len.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), O.data_ptr(),
+            L.data_ptr(), B, Hq, Hkv, D, page_size, max_prefix, max_pages, num_pages,
+            D ** -0.5 if scale is None else scale, raw))
+        if code:
+            self.check_error(code)
+        return O, L
+
+    @staticmethod
+    def _outputs(q, o_shape, l_shape, O, L):
+        """O like q and L fp32, checked where the caller gave them."""
+        import torch
+
+        device = q.get_device()
+        if O is None:
+            O = torch.empty_like(q)
+        else:
+            if O.shape != o_shape:
+                raise _mismatch("O", O, o_shape)
+            _check_packed(q.dtype, O=O)
+            _check_device(device, O)
+        if L is None:
+            L = torch.empty(l_shape, device=q.device, dtype=torch.float32)
+        else:
+            if L.shape != l_shape:
+                raise _mismatch("L", L, l_shape)
+            _check_packed(torch.float32, L=L)
+            _check_device(device, L)
         return O, L
 
     def forward_gqa(self, Q, K, V, causal: bool = False, scale: Optional[float] = None, O=None,
