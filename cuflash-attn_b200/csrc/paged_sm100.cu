@@ -571,76 +571,68 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
         } else if (warp == 1) {
             // ------------------------------------------------ MMA issuer
-            // The whole warp walks the steps (the zeroing of a block's dead V
-            // rows takes all lanes); lane 0 issues.
-            constexpr uint32_t idesc_qk = make_idesc(DType<T>::kMmaFmt, 128, 128, false, false);
-            constexpr uint32_t idesc_pv = make_idesc(DType<T>::kMmaFmt, 128, D, false, true);
-            constexpr uint32_t idesc_kq = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, false, false);
-            constexpr uint32_t idesc_vp = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, true, false);
-            enum { kAcc = 1, kLast = 2, kFreeV = 4, kTransposed = 8, kFreeQ = 16, kQSlot1 = 32 };
-            struct Step {
-                uint32_t v;  // ring fill of its V block
-                int live;    // live keys of the block; -1: already looked after
-                int flags;
-            };
-            uint32_t q_cnt[2] = {0u, 0u};
-            uint32_t p_cnt[2] = {0u, 0u};
-            uint32_t n_s = 0, n_o = 0;  // steps issued
-            uint32_t g0 = 0;            // blocks before the current segment
-            int k = 0, qs = 0, cur_q = 0;
-            int i = 0, steps = 0, n_blk = 0, mode = 0, len = 0, blk0 = 0;
-            bool q_due = false;  // the segment's query tiles are not waited for yet
-            enum { kEnd, kIssued, kStalled };
-            auto next_s = [&](Step& st) -> int {
-                if (i == steps) {
-                    const bool after_few = mode == kFew;
-                    g0 += n_blk;
-                    ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return kEnd;
-                    const Seg& sg = segs[k % kSegRing];
-                    n_blk = sg.n_blk;
-                    mode = sg.mode;
-                    len = sg.len;
-                    blk0 = sg.blk0;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
-                    ++k;
-                    if (n_blk == 0) return kEnd;
-                    since = tick();
-                    i = 0;
-                    steps = mode == kTwoTiles ? 2 * n_blk : n_blk;
-                    q_due = true;
-                    // both query slots are needed, and the few-rows segment before
-                    // holds its own until its last product, which is not issued yet
-                    if (after_few && mode == kTwoTiles && n_s != n_o) return kStalled;
-                }
-                if (q_due) {
-                    q_due = false;
-                    if (mode == kTwoTiles) {
-                        ok = poll(bar_q, q_cnt[0] & 1) &&
-                             poll(bar_q + 1, q_cnt[1] & 1);
-                        ++q_cnt[0];
-                        ++q_cnt[1];
-                    } else {
-                        cur_q = qs;
-                        ok = poll(bar_q + qs, (qs ? q_cnt[1] : q_cnt[0]) & 1);
-                        if (qs) ++q_cnt[1]; else ++q_cnt[0];
-                        qs ^= 1;
+            if (lane == 0) {
+                constexpr uint32_t idesc_qk = make_idesc(DType<T>::kMmaFmt, 128, 128, false, false);
+                constexpr uint32_t idesc_pv = make_idesc(DType<T>::kMmaFmt, 128, D, false, true);
+                constexpr uint32_t idesc_kq = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, false, false);
+                constexpr uint32_t idesc_vp = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, true, false);
+                enum { kAcc = 1, kLast = 2, kFreeV = 4, kTransposed = 8, kFreeQ = 16, kQSlot1 = 32 };
+                struct Step {
+                    uint32_t v;  // ring fill of its V block
+                    int flags;
+                };
+                uint32_t q_cnt[2] = {0u, 0u};
+                uint32_t p_cnt[2] = {0u, 0u};
+                uint32_t n_s = 0, n_o = 0;  // steps issued
+                uint32_t g0 = 0;            // blocks before the current segment
+                int k = 0, qs = 0, cur_q = 0;
+                int i = 0, steps = 0, n_blk = 0, mode = 0;
+                bool q_due = false;  // the segment's query tiles are not waited for yet
+                enum { kEnd, kIssued, kStalled };
+                auto next_s = [&](Step& st) -> int {
+                    if (i == steps) {
+                        const bool after_few = mode == kFew;
+                        g0 += n_blk;
+                        ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
+                        if (!ok) return kEnd;
+                        const Seg& sg = segs[k % kSegRing];
+                        n_blk = sg.n_blk;
+                        mode = sg.mode;
+                        mbar_arrive(seg_free + k % kSegRing);
+                        ++k;
+                        if (n_blk == 0) return kEnd;
+                        since = tick();
+                        i = 0;
+                        steps = mode == kTwoTiles ? 2 * n_blk : n_blk;
+                        q_due = true;
+                        // both query slots are needed, and the few-rows segment before
+                        // holds its own until its last product, which is not issued yet
+                        if (after_few && mode == kTwoTiles && n_s != n_o) return kStalled;
                     }
-                }
-                const bool two = mode == kTwoTiles;
-                const int j = two ? i >> 1 : i;
-                const int u = two ? i & 1 : 0;
-                const uint32_t kf = 2 * (g0 + j);
-                const int s = kf % R;
-                const int t = n_s & 1;
-                if (ok && u == 0) ok = poll(full + s, (kf / R) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return kEnd;
-                const int qslot = two ? u : cur_q;
-                const bool last_in_seg = two ? j == n_blk - 1 : i == steps - 1;
-                if (lane == 0) {
+                    if (q_due) {
+                        q_due = false;
+                        if (mode == kTwoTiles) {
+                            ok = poll(bar_q, q_cnt[0] & 1) &&
+                                 poll(bar_q + 1, q_cnt[1] & 1);
+                            ++q_cnt[0];
+                            ++q_cnt[1];
+                        } else {
+                            cur_q = qs;
+                            ok = poll(bar_q + qs, (qs ? q_cnt[1] : q_cnt[0]) & 1);
+                            if (qs) ++q_cnt[1]; else ++q_cnt[0];
+                            qs ^= 1;
+                        }
+                    }
+                    const bool two = mode == kTwoTiles;
+                    const int j = two ? i >> 1 : i;
+                    const int u = two ? i & 1 : 0;
+                    const uint32_t kf = 2 * (g0 + j);
+                    const int s = kf % R;
+                    const int t = n_s & 1;
+                    if (ok && u == 0) ok = poll(full + s, (kf / R) & 1);
+                    if (!ok) return kEnd;
+                    const int qslot = two ? u : cur_q;
+                    const bool last_in_seg = two ? j == n_blk - 1 : i == steps - 1;
                     tc_fence_after();
                     uint64_t a0 = pg_kdesc<D>(sbase + qslot * G::kQSlotBytes);
                     uint64_t b0 = pg_kdesc<D>(sbase + G::kOffRing + s * G::kTileBytes);
@@ -659,49 +651,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_commit(bar_s + t);
                     if (!two || u == 1) tc_commit(empty + s);
                     if (last_in_seg && mode != kFew) tc_commit(bar_qfree + qslot);
-                }
-                __syncwarp();
-                st.v = kf + 1;
-                st.live = u == 0 ? max(len - (blk0 + j) * kBlockKeys, 0) : -1;
-                st.flags = ((two ? j > 0 : i >= 2) ? kAcc : 0) |
-                           ((two ? j == n_blk - 1 : i + 2 >= steps) ? kLast : 0) |
-                           ((!two || u == 1) ? kFreeV : 0) |
-                           (mode == kFew ? kTransposed | (last_in_seg ? kFreeQ : 0) : 0) |
-                           (qslot ? kQSlot1 : 0);
-                ++i;
-                ++n_s;
-                return kIssued;
-            };
-            auto do_o = [&](const Step& st) -> bool {
-                const int t = n_o & 1;
-                const int s = st.v % R;
-                const uint32_t vbase = sbase + G::kOffRing + s * G::kTileBytes;
-                ok = poll(full + s, (st.v / R) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return false;
-                if (st.live >= 0 && st.live < kBlockKeys) {
-                    // rows behind the context's end hold whatever the page (or the
-                    // ring) had; zero them so that P = 0 meets no NaN
-                    constexpr int kChunks = G::kSwz / 16;
-                    const int n = (kBlockKeys - st.live) * kChunks;
-#pragma unroll
-                    for (int cb = 0; cb < G::kNumCb; ++cb)
-                        for (int e = lane; e < n; e += 32) {
-                            const uint32_t a = vbase + cb * G::kCbBytes + st.live * G::kSwz + e * 16;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
-                        }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                uint64_t v0 = pg_vdesc<D>(vbase);
-                asm volatile("" : "+l"(v0));
-                const uint32_t o_tmem = tmem + 256 + t * 128;
-                const uint32_t par = (t ? p_cnt[1] : p_cnt[0]) & 1;
-                ok = poll(bar_p + t, par);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return false;
-                if (G::kHasFew && (st.flags & kTransposed)) {
-                    if (lane == 0) {
+                    st.v = kf + 1;
+                    st.flags = ((two ? j > 0 : i >= 2) ? kAcc : 0) |
+                               ((two ? j == n_blk - 1 : i + 2 >= steps) ? kLast : 0) |
+                               ((!two || u == 1) ? kFreeV : 0) |
+                               (mode == kFew ? kTransposed | (last_in_seg ? kFreeQ : 0) : 0) |
+                               (qslot ? kQSlot1 : 0);
+                    ++i;
+                    ++n_s;
+                    return kIssued;
+                };
+                auto do_o = [&](const Step& st) -> bool {
+                    const int t = n_o & 1;
+                    const int s = st.v % R;
+                    const uint32_t vbase = sbase + G::kOffRing + s * G::kTileBytes;
+                    ok = poll(full + s, (st.v / R) & 1);
+                    if (!ok) return false;
+                    uint64_t v0 = pg_vdesc<D>(vbase);
+                    asm volatile("" : "+l"(v0));
+                    const uint32_t o_tmem = tmem + 256 + t * 128;
+                    const uint32_t par = (t ? p_cnt[1] : p_cnt[0]) & 1;
+                    ok = poll(bar_p + t, par);
+                    if (!ok) return false;
+                    if (G::kHasFew && (st.flags & kTransposed)) {
                         tc_fence_after();
                         const uint32_t q_off = (st.flags & kQSlot1) ? G::kQSlotBytes : 0;
                         const uint64_t p0 = make_smem_desc(sbase + q_off + G::kOffPt + t * G::kPtBytes, 16, 1024,
@@ -710,58 +682,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int kk = 0; kk < 8; ++kk)
                             mma_f16_ss(o_tmem, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
                                        ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
-                    }
-                    __syncwarp();
-                } else {
-                    if (lane == 0) {
+                    } else {
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
                                        ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
-                    }
-                    __syncwarp();
-                    ok = poll(bar_p2 + t, par);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return false;
-                    if (lane == 0) {
+                        ok = poll(bar_p2 + t, par);
+                        if (!ok) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk)
                             mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
                     }
-                    __syncwarp();
-                }
-                if (lane == 0) {
                     if (st.flags & kLast) tc_commit(bar_o + t);
                     if (st.flags & kFreeV) tc_commit(empty + s);
                     if (st.flags & kFreeQ) tc_commit(bar_qfree + ((st.flags & kQSlot1) ? 1 : 0));
+                    if (t) ++p_cnt[1]; else ++p_cnt[0];
+                    ++n_o;
+                    return true;
+                };
+                Step a, b;
+                int ahead = 0;  // steps whose S is issued and whose O is not (a, then b)
+                bool end = false;
+                while (true) {
+                    while (ahead < 2 && !end) {
+                        const int got = next_s(ahead == 0 ? a : b);
+                        if (got == kStalled) break;
+                        if (got == kEnd)
+                            end = true;
+                        else
+                            ++ahead;
+                    }
+                    if (!ok || (ahead == 0 && end)) break;
+                    if (ahead == 0) continue;
+                    if (!do_o(a)) break;
+                    a = b;
+                    --ahead;
                 }
-                __syncwarp();
-                if (t) ++p_cnt[1]; else ++p_cnt[0];
-                ++n_o;
-                return true;
-            };
-            Step a, b;
-            int ahead = 0;  // steps whose S is issued and whose O is not (a, then b)
-            bool end = false;
-            while (true) {
-                while (ahead < 2 && !end) {
-                    const int got = next_s(ahead == 0 ? a : b);
-                    if (got == kStalled) break;
-                    if (got == kEnd)
-                        end = true;
-                    else
-                        ++ahead;
-                }
-                if (!ok || (ahead == 0 && end)) break;
-                if (ahead == 0) continue;
-                if (!do_o(a)) break;
-                a = b;
-                --ahead;
-            }
-            // all products (and their commits) retire before teardown
-            if (lane == 0) {
+                // all products (and their commits) retire before teardown
                 tc_commit(bar_done);
                 volatile int never = 0;
                 mbar_wait(bar_done, 0, &never, &g_paged_status);
@@ -809,6 +768,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t n0 = 0;  // steps before the segment (its parity matters)
         int qs = 0;       // query slot of the next segment of one tile
         bool y_pending = false;
+        uint32_t g0 = 0;  // key blocks before the segment
+        // Rows behind the context's end hold whatever the page (or the ring)
+        // had: this thread's V row is zeroed so that P = 0 meets no NaN.  The
+        // block's V fill is waited for here; its slot's fill before that one was
+        // read by a step at least two back, so the parity is not ambiguous.
+        auto clean_v = [&](uint32_t fill, int live) -> bool {
+            ok = __all_sync(0xffffffffu, poll(full + fill % R, (fill / R) & 1));
+            if (ok && r >= live) {
+                const uint32_t row = sbase + G::kOffRing + (fill % R) * G::kTileBytes + r * G::kSwz;
+#pragma unroll
+                for (int e = 0; e < G::kRowBytes / 16; ++e)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                     row + (e * 16 / G::kSwz) * G::kCbBytes + e * 16 % G::kSwz),
+                                 "r"(0u)
+                                 : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            return ok;
+        };
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
             ok = __all_sync(0xffffffffu, poll(bar, parity));
             return ok;
@@ -855,6 +833,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                 }
+                if (key0 + kBlockKeys > sg.len &&
+                    !clean_v(2 * (g0 + first + 2 * j) + 1, sg.len - key0))
+                    return;
                 float* rm = rmax + (j & 1) * (4 * kFewRows);
                 float mx[NC];
 #pragma unroll
@@ -994,9 +975,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_arrive(bar_y);
             }
         };
+        int blocks = 0;  // of the last segment
         for (int k = 0; ok; ++k) {
             if (!wait(seg_full + k % kSegRing, (k / kSegRing) & 1)) break;
             const Seg sg = segs[k % kSegRing];
+            g0 += blocks;
+            blocks = sg.n_blk;
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
             if (sg.n_blk == 0) break;
@@ -1033,6 +1017,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!wait(bar_y, (x_cnt - 1) & 1)) break;
                     y_pending = false;
                 }
+                const int in_seg = two ? j : first + 2 * j;  // key block
+                const int col0 = (sg.blk0 + in_seg) * kBlockKeys;
+                // (two tiles: tile 0's product is issued before tile 1's)
+                if (col0 + kBlockKeys > sg.len && tile == 0 &&
+                    !clean_v(2 * (g0 + in_seg) + 1, sg.len - col0))
+                    break;
                 if (!active) {
                     mbar_arrive(bar_p + t);
                     mbar_arrive(bar_p2 + t);
@@ -1041,8 +1031,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_after();
                 uint32_t sr[128];
                 tmem_ld_x128(s_tmem, sr);
-                const int blk = sg.blk0 + (two ? j : first + 2 * j);
-                const int col0 = blk * kBlockKeys;
                 if (col0 + kBlockKeys > sg.len || (ln.causal && col0 + kBlockKeys - 1 > tile_lim)) {
                     const int vis = row_end - col0;  // column i is visible iff i <= vis
 #pragma unroll
@@ -1224,21 +1212,44 @@ struct JoinAcc {
     float tot;
 };
 
+// Adds n partials: row r of the tiles of `rows` rows at base, base + step, ...
 template <int D>
-__device__ __forceinline__ void join_add(const TcParams& p, JoinAcc<D>& a, float M, int base, int rows,
-                                         int r) {
-    const float w = sm100::ex2_approx(p.L_part[base + r] - M);
-    a.tot += w;
-    const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(base) * D) + r +
-                        (threadIdx.x >> 5) * JoinAcc<D>::kQuads * rows;
+__device__ __forceinline__ void join_add(const TcParams& p, JoinAcc<D>& a, float M, int n, int base,
+                                         int step, int rows, int r) {
+    constexpr int Q = JoinAcc<D>::kQuads;
+    constexpr int kFlight = 16 / Q;  // partials in flight: 16 loads of 16 bytes per thread
+    for (int k0 = 0; k0 < n; k0 += kFlight) {
+        float4 s[kFlight][Q];
+        float w[kFlight];
 #pragma unroll
-    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) {
-        const float4 s = src[q * rows];
-        a.v[q].x = fmaf(w, s.x, a.v[q].x);
-        a.v[q].y = fmaf(w, s.y, a.v[q].y);
-        a.v[q].z = fmaf(w, s.z, a.v[q].z);
-        a.v[q].w = fmaf(w, s.w, a.v[q].w);
+        for (int k = 0; k < kFlight; ++k) {
+            const int at = base + min(k0 + k, n - 1) * step;
+            w[k] = p.L_part[at + r];
+            const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(at) * D) + r +
+                                (threadIdx.x >> 5) * Q * rows;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) s[k][q] = src[q * rows];
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const float wk = k0 + k < n ? sm100::ex2_approx(w[k] - M) : 0.f;
+            a.tot += wk;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                a.v[q].x = fmaf(wk, s[k][q].x, a.v[q].x);
+                a.v[q].y = fmaf(wk, s[k][q].y, a.v[q].y);
+                a.v[q].z = fmaf(wk, s[k][q].z, a.v[q].z);
+                a.v[q].w = fmaf(wk, s[k][q].w, a.v[q].w);
+            }
+        }
     }
+}
+
+// Largest log2-sum-exp of n partials (same rows as join_add).
+__device__ __forceinline__ float join_max(const TcParams& p, float M, int n, int base, int step, int r) {
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[base + k * step + r]);
+    return M;
 }
 
 // Writes this block's 32 rows; lane's row goes to out_row (-1: none).
@@ -1304,14 +1315,12 @@ __global__ void __launch_bounds__(kJoinThreads)
     if (!partials_ready()) return;
     PrefixParts q = {};
     if (valid) q = prefix_parts(ln, *ln.per, pre, own, b, hc, hr);
-    float M = -INFINITY;
-    for (int k = 0; k < q.n1; ++k) M = fmaxf(M, p.L_part[q.row1 + k * (2 * kTileRows) + q.r1]);
-    for (int k = 0; k < q.n2; ++k) M = fmaxf(M, p.L_part[q.row2 + k * ln.gt + q.r2]);
+    float M = join_max(p, -INFINITY, q.n1, q.row1, 2 * kTileRows, q.r1);
+    M = join_max(p, M, q.n2, q.row2, ln.gt, q.r2);
     JoinAcc<D> a = join_zero<D>();
     if (M != -INFINITY) {
-#pragma unroll 2
-        for (int k = 0; k < q.n1; ++k) join_add<D>(p, a, M, q.row1 + k * (2 * kTileRows), kTileRows, q.r1);
-        for (int k = 0; k < q.n2; ++k) join_add<D>(p, a, M, q.row2 + k * ln.gt, ln.gt, q.r2);
+        join_add<D>(p, a, M, q.n1, q.row1, 2 * kTileRows, kTileRows, q.r1);
+        join_add<D>(p, a, M, q.n2, q.row2, ln.gt, ln.gt, q.r2);
     }
     join_store<T, D>(p, a, M, valid ? b * ln.hq + hk * ln.group + ch * ln.gt + hr : -1);
 }
@@ -1336,13 +1345,15 @@ __global__ void __launch_bounds__(kJoinThreads)
     const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
     if (__syncthreads_or(valid) == 0) return;
     const int n = valid ? sp.last - i + 1 : 0;
-    auto base = [&](int k) { return (2 * (i + k) + (k == 0 ? 1 : 0)) * (2 * kTileRows) + tile * kTileRows; };
-    float M = -INFINITY;
-    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[base(k) + r]);
+    // CTA i's last piece, then the first ones of the CTAs behind it
+    const int base0 = (2 * i + 1) * (2 * kTileRows) + tile * kTileRows;
+    const int base1 = (2 * i + 2) * (2 * kTileRows) + tile * kTileRows;
+    float M = join_max(p, -INFINITY, min(n, 1), base0, 0, r);
+    M = join_max(p, M, n - 1, base1, 4 * kTileRows, r);
     JoinAcc<D> a = join_zero<D>();
     if (M != -INFINITY) {
-#pragma unroll 2
-        for (int k = 0; k < n; ++k) join_add<D>(p, a, M, base(k), kTileRows, r);
+        join_add<D>(p, a, M, min(n, 1), base0, 0, kTileRows, r);
+        join_add<D>(p, a, M, n - 1, base1, 4 * kTileRows, kTileRows, r);
     }
     join_store<T, D>(p, a, M, valid ? token * ln.hq + sp.head0 + hr : -1);
 }
