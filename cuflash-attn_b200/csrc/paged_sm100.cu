@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -305,6 +306,51 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Converged-warp forms of the tcgen05 instructions: issued by the lane whose
+// `leader` is set (elect_lane, once per role).
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p;
+}
+template <typename V>
+__device__ __forceinline__ V uniform(V v) {
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
+            sm100::smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+
 __device__ __forceinline__ float warp_max(float v) {
     float m;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
@@ -456,6 +502,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (*abort_flag || tick() - since > kWaitTicks) return false;
         return true;
     };
+    // The same for waits that are not urgent: a polling warp takes issue slots
+    // from the softmax warps of its quarter.
+    auto poll_idle = [&](uint64_t* bar, uint32_t parity, unsigned ns) -> bool {
+        const uint32_t addr = smem_u32(bar);
+        while (!mbar_try_wait(addr, parity)) {
+            if (*abort_flag || tick() - since > kWaitTicks) return false;
+            __nanosleep(ns);
+        }
+        return true;
+    };
 
     // Registers: launched with 168 per thread (384 x 168 = 64512); the first
     // warpgroup gives back down to 72 and the two softmax warpgroups take 216:
@@ -503,7 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
                         const int slot = sg.mode == kTwoTiles ? u : qs;
                         if (q_cnt[slot] > 0)
-                            ok = poll(bar_qfree + slot, (q_cnt[slot] - 1) & 1);
+                            ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20);
                         if (!ok) break;
                         mbar_arrive_expect_tx(bar_q + slot, bytes);
                         for (int cb = 0; cb < G::kNumCb; ++cb)
@@ -543,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const int s = kv % R;
                         if (lane == 0) {
                             if (kv >= static_cast<uint32_t>(R))
-                                ok = poll(empty + s, (kv / R - 1) & 1);
+                                ok = poll_idle(empty + s, (kv / R - 1) & 1, 20);
                             if (ok)
                                 mbar_arrive_expect_tx(full + s, static_cast<uint32_t>(nbox * box_rows) *
                                                                     G::kRowBytes);
@@ -571,157 +627,163 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
         } else if (warp == 1) {
             // ------------------------------------------------ MMA issuer
-            if (lane == 0) {
+            // The warp stays converged and one elected lane issues: every value a
+            // product takes is then warp-uniform for the compiler (registers of
+            // the uniform datapath, no per-thread copies before each instruction).
+            // What it spends between products is on every step's critical path,
+            // so the steps are unrolled over the two streams, ring positions are
+            // counted up, and a step waiting for its O is one word of flags.
+            {
+                const uint32_t leader = elect_lane();
+                const uint32_t tm = uniform(tmem);
+                const uint32_t sb = uniform(sbase);
+                auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                    ok = __all_sync(0xffffffffu, poll(bar, parity));
+                    return ok;
+                };
                 constexpr uint32_t idesc_qk = make_idesc(DType<T>::kMmaFmt, 128, 128, false, false);
                 constexpr uint32_t idesc_pv = make_idesc(DType<T>::kMmaFmt, 128, D, false, true);
                 constexpr uint32_t idesc_kq = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, false, false);
                 constexpr uint32_t idesc_vp = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, true, false);
-                enum { kAcc = 1, kLast = 2, kFreeV = 4, kTransposed = 8, kFreeQ = 16, kQSlot1 = 32 };
-                struct Step {
-                    uint32_t v;  // ring fill of its V block
-                    int flags;
-                };
-                uint32_t q_cnt[2] = {0u, 0u};
-                uint32_t p_cnt[2] = {0u, 0u};
-                uint32_t n_s = 0, n_o = 0;  // steps issued
-                uint32_t g0 = 0;            // blocks before the current segment
+                constexpr uint32_t kDue = 1, kAcc = 2, kLast = 4, kWaitV = 8, kFreeV = 16, kIsFew = 32,
+                                   kFreeQ = 64, kQSlot1 = 128;
+                uint32_t ks = 0, kph = 0;  // ring slot and phase of the next block's K
+                uint32_t vs = 1, vph = 0;  // of the V of the step whose O is next
+                uint32_t due0 = 0, due1 = 0;  // each stream's step that has its S but not its O
+                uint32_t par0 = 0, par1 = 0;  // phases of bar_p
+                uint32_t qph = 0;             // bit u: phase of bar_q[u]
                 int k = 0, qs = 0, cur_q = 0;
-                int i = 0, steps = 0, n_blk = 0, mode = 0;
-                bool q_due = false;  // the segment's query tiles are not waited for yet
-                enum { kEnd, kIssued, kStalled };
-                auto next_s = [&](Step& st) -> int {
-                    if (i == steps) {
-                        const bool after_few = mode == kFew;
-                        g0 += n_blk;
-                        ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
-                        if (!ok) return kEnd;
-                        const Seg& sg = segs[k % kSegRing];
-                        n_blk = sg.n_blk;
-                        mode = sg.mode;
-                        mbar_arrive(seg_free + k % kSegRing);
-                        ++k;
-                        if (n_blk == 0) return kEnd;
-                        since = tick();
-                        i = 0;
-                        steps = mode == kTwoTiles ? 2 * n_blk : n_blk;
-                        q_due = true;
-                        // both query slots are needed, and the few-rows segment before
-                        // holds its own until its last product, which is not issued yet
-                        if (after_few && mode == kTwoTiles && n_s != n_o) return kStalled;
+                int i = 0, steps = 0, mode = kTwoTiles;
+                bool end = false;
+                auto next_slot = [](uint32_t& s, uint32_t& ph) {
+                    s += 2;
+                    if (s >= R) {
+                        s -= R;
+                        ph ^= 1;
                     }
-                    if (q_due) {
-                        q_due = false;
+                };
+                // S of the next step (stream t); its flags, 0 at the end
+                auto issue_s = [&](auto stream) -> uint32_t {
+                    constexpr int t = decltype(stream)::value;
+                    if (i == steps) {
+                        if (!wait(seg_full + k % kSegRing, (k / kSegRing) & 1)) return 0;
+                        const Seg& sg = segs[k % kSegRing];
+                        steps = uniform(sg.n_blk);
+                        mode = uniform(sg.mode);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
+                        ++k;
+                        i = 0;
+                        end = steps == 0;
+                        if (end) return 0;
+                        since = tick();
                         if (mode == kTwoTiles) {
-                            ok = poll(bar_q, q_cnt[0] & 1) &&
-                                 poll(bar_q + 1, q_cnt[1] & 1);
-                            ++q_cnt[0];
-                            ++q_cnt[1];
+                            steps *= 2;
+                            if (!wait(bar_q, qph & 1) || !wait(bar_q + 1, qph >> 1)) return 0;
+                            qph ^= 3;
                         } else {
                             cur_q = qs;
-                            ok = poll(bar_q + qs, (qs ? q_cnt[1] : q_cnt[0]) & 1);
-                            if (qs) ++q_cnt[1]; else ++q_cnt[0];
+                            if (!wait(bar_q + qs, (qph >> qs) & 1)) return 0;
+                            qph ^= 1u << qs;
                             qs ^= 1;
                         }
                     }
                     const bool two = mode == kTwoTiles;
-                    const int j = two ? i >> 1 : i;
                     const int u = two ? i & 1 : 0;
-                    const uint32_t kf = 2 * (g0 + j);
-                    const int s = kf % R;
-                    const int t = n_s & 1;
-                    if (ok && u == 0) ok = poll(full + s, (kf / R) & 1);
-                    if (!ok) return kEnd;
+                    if (u == 0 && !wait(full + ks, kph)) return 0;
                     const int qslot = two ? u : cur_q;
-                    const bool last_in_seg = two ? j == n_blk - 1 : i == steps - 1;
                     tc_fence_after();
-                    uint64_t a0 = pg_kdesc<D>(sbase + qslot * G::kQSlotBytes);
-                    uint64_t b0 = pg_kdesc<D>(sbase + G::kOffRing + s * G::kTileBytes);
-                    asm volatile("" : "+l"(a0), "+l"(b0));
+                    const uint64_t a0 = pg_kdesc<D>(sb + qslot * G::kQSlotBytes);
+                    const uint64_t b0 = pg_kdesc<D>(sb + G::kOffRing + ks * G::kTileBytes);
+                    uint32_t flags = kDue | (i >= 2 ? kAcc : 0) | (i + 2 >= steps ? kLast : 0);
                     if (G::kHasFew && mode == kFew) {
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            mma_f16_ss(tmem + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
+                            mma_ss(leader, tm + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
                                        kk > 0 ? 1u : 0u);
+                        flags |= kIsFew | (qslot ? kQSlot1 : 0) | (i + 1 == steps ? kFreeQ : 0);
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            mma_f16_ss(tmem + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
+                            mma_ss(leader, tm + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
                                        kk > 0 ? 1u : 0u);
                     }
-                    tc_commit(bar_s + t);
-                    if (!two || u == 1) tc_commit(empty + s);
-                    if (last_in_seg && mode != kFew) tc_commit(bar_qfree + qslot);
-                    st.v = kf + 1;
-                    st.flags = ((two ? j > 0 : i >= 2) ? kAcc : 0) |
-                               ((two ? j == n_blk - 1 : i + 2 >= steps) ? kLast : 0) |
-                               ((!two || u == 1) ? kFreeV : 0) |
-                               (mode == kFew ? kTransposed | (last_in_seg ? kFreeQ : 0) : 0) |
-                               (qslot ? kQSlot1 : 0);
+                    commit(leader, bar_s + t);
+                    if (two) {
+                        if (i + 2 >= steps) commit(leader, bar_qfree + u);
+                        flags |= u ? kFreeV : kWaitV;
+                    } else {
+                        if (i + 1 == steps && mode != kFew) commit(leader, bar_qfree + cur_q);
+                        flags |= kFreeV | kWaitV;
+                    }
+                    if (flags & kFreeV) {
+                        commit(leader, empty + ks);
+                        next_slot(ks, kph);
+                    }
                     ++i;
-                    ++n_s;
-                    return kIssued;
+                    return flags;
                 };
-                auto do_o = [&](const Step& st) -> bool {
-                    const int t = n_o & 1;
-                    const int s = st.v % R;
-                    const uint32_t vbase = sbase + G::kOffRing + s * G::kTileBytes;
-                    ok = poll(full + s, (st.v / R) & 1);
-                    if (!ok) return false;
-                    uint64_t v0 = pg_vdesc<D>(vbase);
-                    asm volatile("" : "+l"(v0));
-                    const uint32_t o_tmem = tmem + 256 + t * 128;
-                    const uint32_t par = (t ? p_cnt[1] : p_cnt[0]) & 1;
-                    ok = poll(bar_p + t, par);
-                    if (!ok) return false;
-                    if (G::kHasFew && (st.flags & kTransposed)) {
-                        tc_fence_after();
-                        const uint32_t q_off = (st.flags & kQSlot1) ? G::kQSlotBytes : 0;
-                        const uint64_t p0 = make_smem_desc(sbase + q_off + G::kOffPt + t * G::kPtBytes, 16, 1024,
-                                                           kLayoutSw128);
+                // O of stream t's step, in step order
+                auto issue_o = [&](auto stream, uint32_t flags) -> bool {
+                    constexpr int t = decltype(stream)::value;
+                    uint32_t& par = t ? par1 : par0;
+                    if ((flags & kWaitV) && !wait(full + vs, vph)) return false;
+                    if (!wait(bar_p + t, par)) return false;
+                    const uint64_t v0 = pg_vdesc<D>(sb + G::kOffRing + vs * G::kTileBytes);
+                    constexpr int kO = 256 + t * 128;
+                    const uint32_t acc = (flags & kAcc) ? 1u : 0u;
+                    tc_fence_after();
+                    if (G::kHasFew && (flags & kIsFew)) {
+                        const uint32_t q_off = (flags & kQSlot1) ? G::kQSlotBytes : 0;
+                        const uint64_t p0 = make_smem_desc(sb + q_off + G::kOffPt + t * G::kPtBytes, 16, 1024,
+                                                     kLayoutSw128);
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_f16_ss(o_tmem, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
-                                       ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
+                            mma_ss(leader, tm + kO, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
+                                       kk > 0 ? 1u : acc);
+                        if (flags & kFreeQ) commit(leader, bar_qfree + ((flags & kQSlot1) ? 1 : 0));
                     } else {
-                        tc_fence_after();
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
-                                       ((st.flags & kAcc) || kk > 0) ? 1u : 0u);
-                        ok = poll(bar_p2 + t, par);
-                        if (!ok) return false;
+                            mma_ts(leader, tm + kO, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
+                                       kk > 0 ? 1u : acc);
+                        if (!wait(bar_p2 + t, par)) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk)
-                            mma_f16_ts(o_tmem, tmem + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
+                            mma_ts(leader, tm + kO, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
                     }
-                    if (st.flags & kLast) tc_commit(bar_o + t);
-                    if (st.flags & kFreeV) tc_commit(empty + s);
-                    if (st.flags & kFreeQ) tc_commit(bar_qfree + ((st.flags & kQSlot1) ? 1 : 0));
-                    if (t) ++p_cnt[1]; else ++p_cnt[0];
-                    ++n_o;
+                    if (flags & kLast) commit(leader, bar_o + t);
+                    if (flags & kFreeV) {
+                        commit(leader, empty + vs);
+                        next_slot(vs, vph);
+                    }
+                    par ^= 1;
                     return true;
                 };
-                Step a, b;
-                int ahead = 0;  // steps whose S is issued and whose O is not (a, then b)
-                bool end = false;
-                while (true) {
-                    while (ahead < 2 && !end) {
-                        const int got = next_s(ahead == 0 ? a : b);
-                        if (got == kStalled) break;
-                        if (got == kEnd)
-                            end = true;
-                        else
-                            ++ahead;
+                // Stream t's turn: its O, then its next S behind it (in order, so
+                // that S may overwrite P).  With few rows the loads set the pace: the
+                // other stream's O does not wait behind an S whose keys have not
+                // landed; and the segment's products end before the next segment
+                // begins, which may need the query slot that holds P^T.
+                auto turn = [&](auto stream, uint32_t& due, uint32_t& other) -> bool {
+                    constexpr int t = decltype(stream)::value;
+                    std::integral_constant<int, t ^ 1> next;
+                    if (due != 0 && !issue_o(stream, due)) return false;
+                    due = 0;
+                    if (G::kHasFew && mode == kFew && other != 0 &&
+                        (i == steps || !__all_sync(0xffffffffu, mbar_test(full + ks, kph)))) {
+                        if (!issue_o(next, other)) return false;
+                        other = 0;
                     }
-                    if (!ok || (ahead == 0 && end)) break;
-                    if (ahead == 0) continue;
-                    if (!do_o(a)) break;
-                    a = b;
-                    --ahead;
+                    if (!end) due = issue_s(stream);
+                    return ok;
+                };
+                while (turn(std::integral_constant<int, 0>(), due0, due1) &&
+                       turn(std::integral_constant<int, 1>(), due1, due0) && (due0 | due1) != 0) {
                 }
                 // all products (and their commits) retire before teardown
-                tc_commit(bar_done);
+                commit(leader, bar_done);
                 volatile int never = 0;
                 mbar_wait(bar_done, 0, &never, &g_paged_status);
             }
@@ -732,7 +794,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 int k = 0;
                 auto emit = [&](const Seg& sg) {
                     if (k >= kSegRing)
-                        ok = poll(seg_free + k % kSegRing, (k / kSegRing - 1) & 1);
+                        ok = poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500);
                     if (!ok) return;
                     since = tick();
                     segs[k % kSegRing] = sg;
