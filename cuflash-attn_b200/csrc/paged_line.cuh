@@ -8,15 +8,25 @@
 // one K/V head (in chunks of gt <= 128 of them) are packed with the tokens
 // into row tiles of tpt tokens x gt heads <= 128 rows, so that every key and
 // value is read once for all of them.  A unit is one head chunk with two row
-// tiles, with one where no second is left, or with few rows (at most kFewRows
-// in the whole context).  Its length is its number of 128-key blocks, weighted
-// by the kind of unit.  The units' lengths, one after the other (context, then
-// head chunk, then row tiles), form a line that is cut into pieces of `per`,
-// one per CTA.  The lengths live in device memory, so every CTA works out the
-// line itself, in closed form per context.  A piece that covers a whole ragged
-// unit writes the result; all others write partials for a second kernel.
+// tiles, with one where no second is left, or with few rows (at most few_rows
+// in the whole context).  Its length is the number of keys its last token
+// sees plus kUnitCost, doubled for two tiles; key block j (128 keys) lies at
+// 128 j of it.  The units, one after the other (context, then head chunk, then
+// row tiles), form a line that is cut into equal pieces, one per CTA.  There
+// are two lines: units of row tiles, which the tensor cores bound, and units
+// of few rows, which the loads of keys and values bound; CTA i takes piece i
+// of the first and piece G - 1 - i of the second, so that few pieces of either
+// kind do not meet on the same CTAs.  The lengths live in device memory, so
+// every CTA works out the lines itself, in closed form per context (lengths
+// linear in the keys rather than counted in blocks make the sum over a
+// context's causal units an arithmetic series).  A piece that covers a whole
+// ragged unit writes the result; all others write partials for a second
+// kernel, and the piece with a unit's first block records which pieces those
+// are.
 //
-// Plain integer code, host and device.
+// Plain integer code, host and device; small on purpose: the kernel's roles
+// share the instruction caches, and unrolled or repeated copies of this code
+// (divisions above all) made up a third of it.
 
 #include <cuda_runtime.h>
 
@@ -28,7 +38,20 @@ namespace detail {
 constexpr int kTileRows = 128;
 constexpr int kBlockKeys = 128;
 
+constexpr int kFewTile = 16;  // rows of a partial tile of few rows (ragged)
+
+#ifdef __CUDACC__
+#define CUFLASH_ROLLED _Pragma("unroll 1")
+#else
+#define CUFLASH_ROLLED
+#endif
+
+// What a unit costs besides its keys, in keys: with 127, a unit of row tiles
+// weighs as much as its key blocks.
+constexpr int kUnitCost = 127;
+
 enum UnitMode { kOneTile = 0, kTwoTiles = 1, kFew = 2 };
+enum Line { kTiles = 0, kFewLine = 1 };
 
 // One CTA's part of one unit.
 struct Seg {
@@ -49,9 +72,13 @@ struct Seg {
 };
 static_assert(sizeof(Seg) == 64, "Seg layout");
 
-// A ragged unit whose blocks several CTAs share: written by the first.
+// The pieces of a unit: written by the one with its first block.  Prefix decode:
+// of every unit; ragged: of the units that several pieces share, by piece.
+struct Span {
+    int first, last;
+};
 struct Split {
-    int last;  // last CTA of the unit, -1: none
+    int last;  // last piece of the unit, -1: none
     int tok0, tok_end, head0, nh, mode;
     int pad[2];
 };
@@ -63,137 +90,156 @@ struct PagedLine {
     int prefix_mode, causal;
     int num_tokens, B, hq, hkv, group;
     int gt, chunks, tpt;  // heads per tile, chunks of the group, tokens per tile
+    int heads;            // head chunks: hkv * chunks
     int few_rows;         // contexts of at most this many rows are "few"
     int page_shift, max_prefix_pages, max_pages;
-    int w_two, w_one, w_few;  // line length of a block
-    int min_per;              // shortest piece, at least the largest weight
-    int own_part_row;         // first partial row of the own-keys units
-    int* per;                 // piece length, for the second kernel
-    int* unit_start;          // prefix decode: line position of own-keys unit u
-    Split* split;             // ragged: one per CTA
+    int prefix_pairs;  // units per head chunk of the prefix
+    int pieces;        // of each line: the CTAs of the launch
+    int own_part_row;  // prefix decode: first partial row of the own-keys units
+    int few_part_row;  // ragged: first partial row of units of few rows
+    Span* span;        // prefix decode: [heads * prefix_pairs] prefix units, [B * heads] own
+    Split* split;      // ragged: one per piece of each line
 };
-
-// sum over i in [0, n) of floor((a i + b) / m): the usual Euclid-like
-// reduction (a, b >= 0, m > 0; n, m and b mod m small enough for 32 bits).
-__host__ __device__ __forceinline__ int floor_sum(int n, int m, int a, int b) {
-    int s = 0;
-    while (n > 0) {
-        s += static_cast<int>(static_cast<long long>(n) * (n - 1) / 2) * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const int top = a * n + b;
-        n = top / m;
-        b = top % m;
-        const int t = m;
-        m = a;
-        a = t;
-        if (m == 0) break;  // then top < the old m, so n == 0
-    }
-    return s;
-}
 
 struct Ctx {
     int tok, ntok, len;
-    int pairs;      // units per head chunk
-    int last_mode;  // of the last one; the others have two tiles
-    int head_cost;  // line length of a head chunk
+    int pairs;            // units per head chunk
+    int last_mode;        // of the last one; the others have two tiles
+    long long head_cost;  // line length of a head chunk
 };
 
-__host__ __device__ __forceinline__ int unit_blocks(const PagedLine& p, const Ctx& c, int pair) {
-    int vis = c.len;
-    if (p.causal && pair < c.pairs - 1)
-        vis = c.len - c.ntok + (pair + 1) * 2 * p.tpt;  // what its last token sees
-    const int nb = (vis + kBlockKeys - 1) / kBlockKeys;
-    // ragged: a unit that sees no key takes one masked block, which writes its rows
-    return p.prefix_mode ? nb : (vis > 0 ? nb : 1);
+// Keys that the last token of a unit sees, at least 1 (ragged: a unit that sees
+// none takes one masked block, which writes its rows).
+__host__ __device__ __forceinline__ int unit_keys(const PagedLine& p, const Ctx& c, int pair) {
+    int n = c.len;
+    if (p.causal && pair < c.pairs - 1) n += (pair + 1) * 2 * p.tpt - c.ntok;
+    return n > 0 ? n : 1;
 }
 
 __host__ __device__ __forceinline__ int unit_mode(const Ctx& c, int pair) {
     return pair < c.pairs - 1 ? static_cast<int>(kTwoTiles) : c.last_mode;
 }
 
-__host__ __device__ __forceinline__ int mode_weight(const PagedLine& p, int mode) {
-    return mode == kTwoTiles ? p.w_two : (mode == kOneTile ? p.w_one : p.w_few);
+// Line length of the first n (two-tile) units of a head chunk: the sum over
+// i = 1..n of max(off + i s, 1) + kUnitCost, doubled.
+__host__ __device__ __forceinline__ long long pairs_cost(const PagedLine& p, const Ctx& c, int n) {
+    const int s = p.causal ? 2 * p.tpt : 0;
+    const int off = p.causal ? c.len - c.ntok : (c.len > 0 ? c.len : 1);
+    int z = off < 0 ? -off / s : 0;  // units that see no key
+    if (z > n) z = n;
+    const long long m = n - z;
+    const long long steps = (m * (m + 1)) / 2 + m * z;  // z + 1 + ... + n
+    return 2 * (n * static_cast<long long>(kUnitCost) + z + m * off + steps * s);
 }
 
-// Line length of the first `pairs` (two-tile) units of a head chunk.
-__host__ __device__ __forceinline__ int pairs_cost(const PagedLine& p, const Ctx& c, int pairs) {
-    if (pairs == 0) return 0;
-    if (!p.causal) return pairs * unit_blocks(p, c, 0) * p.w_two;
-    const int s = 2 * p.tpt;
-    const int off = c.len - c.ntok;
-    // units whose last token sees at most 128 keys take one block
-    int ones = 128 - off >= 0 ? (128 - off) / s : 0;
-    if (ones > pairs) ones = pairs;
-    return (ones + floor_sum(pairs - ones, 128, s, off + (ones + 1) * s + 127)) * p.w_two;
+__host__ __device__ __forceinline__ long long unit_length(const PagedLine& p, const Ctx& c, int pair) {
+    return static_cast<long long>(unit_keys(p, c, pair) + kUnitCost) << (unit_mode(c, pair) == kTwoTiles);
 }
 
 // Context c: -1 is the shared prefix.
 __host__ __device__ __forceinline__ Ctx load_ctx(const PagedLine& p, int c) {
     Ctx x;
+    const bool shared = c < 0;
+    x.len = clamp_len(shared ? *p.prefix_len : p.seq_lens[c],
+                      (shared ? p.max_prefix_pages : p.max_pages) << p.page_shift);
     if (p.prefix_mode) {
-        x.tok = c < 0 ? 0 : c;
-        x.ntok = c < 0 ? p.B : 1;
-        x.len = c < 0 ? clamp_len(*p.prefix_len, p.max_prefix_pages << p.page_shift)
-                      : clamp_len(p.seq_lens[c], p.max_pages << p.page_shift);
+        x.tok = shared ? 0 : c;
+        x.ntok = shared ? p.B : 1;
     } else {
         x.tok = clamp_len(p.cu_seqlens[c], p.num_tokens);
         x.ntok = clamp_len(p.cu_seqlens[c + 1] - x.tok, p.num_tokens - x.tok);
-        x.len = clamp_len(p.seq_lens[c], p.max_pages << p.page_shift);
     }
     const int tiles = (x.ntok + p.tpt - 1) / p.tpt;
     x.pairs = (tiles + 1) / 2;
     x.last_mode = (tiles & 1) == 0 ? kTwoTiles : (x.ntok * p.gt <= p.few_rows ? kFew : kOneTile);
     x.head_cost = 0;
     if (x.pairs > 0 && (x.len > 0 || !p.prefix_mode))
-        x.head_cost = pairs_cost(p, x, x.pairs - 1) +
-                      unit_blocks(p, x, x.pairs - 1) * mode_weight(p, x.last_mode);
+        x.head_cost = pairs_cost(p, x, x.pairs - 1) + unit_length(p, x, x.pairs - 1);
     return x;
 }
 
-// The piece [x0, x1) of the line that belongs to CTA `cta`, unit by unit.
+// The line of a context's units: those of one context are all of one kind but
+// the last, which has few rows only where it is the only one.
+__host__ __device__ __forceinline__ int line_of(const Ctx& c) {
+    return c.last_mode == kFew ? static_cast<int>(kFewLine) : static_cast<int>(kTiles);
+}
+
+// Length of a piece: at least a block of a two-tile unit, so that every piece
+// between a unit's first and last one has a block of it.
+__host__ __device__ __forceinline__ long long piece_length(long long line, int pieces) {
+    const int shift = line >> 31 ? 20 : 0;
+    const long long per =
+        static_cast<long long>(static_cast<unsigned>(line >> shift) / static_cast<unsigned>(pieces) + 1) << shift;
+    return per < 2 * kBlockKeys ? 2 * kBlockKeys : per;
+}
+
+// y / d for quotients below 2^20: an estimate, put right.
+__host__ __device__ __forceinline__ int quotient(long long y, long long d) {
+#ifdef __CUDA_ARCH__
+    int q = static_cast<int>(__fdividef(static_cast<float>(y), static_cast<float>(d)));
+#else
+    int q = static_cast<int>(static_cast<float>(y) / static_cast<float>(d));
+#endif
+    CUFLASH_ROLLED
+    while (q * d > y) --q;
+    CUFLASH_ROLLED
+    while ((q + 1) * d <= y) ++q;
+    return q;
+}
+
+// Piece [x0, x1) of a line, unit by unit.
 struct Walk {
     Ctx ctx;
-    int c, hc, pair, cta;   // context, head chunk, unit of it
-    int ub, x, x1, per;     // line position of the unit, of the walk, its end
+    int c, hc, pair;           // context, head chunk, unit of it
+    int line, piece, records;  // records: this walk writes them
+    long long ub, x, x0, x1, per;  // line position of the unit, of the walk; the piece; its length
 };
 
 // Context c holds position x0 and starts at ctx_base.
-__host__ __device__ __forceinline__ void walk_start(const PagedLine& p, Walk& w, const Ctx& ctx,
-                                                    int c, int ctx_base, int x0, int x1, int per,
-                                                    int cta) {
+__host__ __device__ __forceinline__ void walk_start(const PagedLine& p, Walk& w, const Ctx& ctx, int c,
+                                                    long long ctx_base, long long x0, long long x1,
+                                                    long long per, int line, int piece, bool records) {
     w.ctx = ctx;
     w.c = c;
-    w.cta = cta;
-    w.x = x0;
+    w.line = line;
+    w.piece = piece;
+    w.records = records;
+    w.x = w.x0 = x0;
     w.x1 = x1;
     w.per = per;
-    const int y = x0 - ctx_base;
-    w.hc = y / ctx.head_cost;
-    const int z = y - w.hc * ctx.head_cost;
-    int lo = 0, hi = ctx.pairs;  // the unit of the head chunk that z falls into
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (pairs_cost(p, ctx, mid) <= z)
+    w.hc = quotient(x0 - ctx_base, ctx.head_cost);
+    const long long base = ctx_base + w.hc * ctx.head_cost;
+    int lo = 0, hi = ctx.pairs - 1;  // the last unit that does not start behind x0
+    w.ub = base;
+    CUFLASH_ROLLED
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        const long long at = base + pairs_cost(p, ctx, mid);
+        if (at <= x0) {
             lo = mid;
-        else
-            hi = mid;
+            w.ub = at;
+        } else {
+            hi = mid - 1;
+        }
     }
     w.pair = lo;
-    w.ub = ctx_base + w.hc * ctx.head_cost + pairs_cost(p, ctx, lo);
 }
 
-// The next segment; false at the end.  Records where own-keys units start and
-// which ragged units several CTAs share, for the second kernel.
-__host__ __device__ __forceinline__ bool walk_next(const PagedLine& p, Walk& w, Seg& sg) {
-    const int heads = p.hkv * p.chunks;
+// The next segment; false at the end.  next_ctx(c, line, ctx): the first
+// context behind c with units on the line.
+template <typename NextCtx>
+__host__ __device__ __forceinline__ bool walk_next(const PagedLine& p, Walk& w, Seg& sg,
+                                                   const NextCtx& next_ctx) {
+    CUFLASH_ROLLED
     while (w.x < w.x1) {
-        const int nb = unit_blocks(p, w.ctx, w.pair);
         const int mode = unit_mode(w.ctx, w.pair);
-        const int wt = mode_weight(p, mode);
-        const int blk0 = (w.x - w.ub + wt - 1) / wt;
-        const int end = (w.x1 - w.ub + wt - 1) / wt;
-        const int blk1 = end < nb ? end : nb;
+        const int keys = unit_keys(p, w.ctx, w.pair);
+        const int nb = (keys + kBlockKeys - 1) / kBlockKeys;
+        const int two = mode == kTwoTiles ? 1 : 0;
+        const int sh = 7 + two;  // line length of a block: 128, doubled
+        const int blk0 = static_cast<int>((w.x - w.ub + (1 << sh) - 1) >> sh);
+        const long long end = (w.x1 - w.ub + (1 << sh) - 1) >> sh;
+        const int blk1 = end < nb ? static_cast<int>(end) : nb;
         const bool some = blk1 > blk0;
         if (some) {
             sg.n_blk = blk1 - blk0;
@@ -209,80 +255,44 @@ __host__ __device__ __forceinline__ bool walk_next(const PagedLine& p, Walk& w, 
             sg.ctx = w.c;
             sg.mode = mode;
             sg.part_rows = kTileRows;
+            const bool first = blk0 == 0;
+            int last = w.piece;
+            if (first && blk1 < nb)
+                last += quotient(w.ub + (static_cast<long long>(nb - 1) << sh) - w.x0, w.per);
             if (p.prefix_mode) {
+                int u = w.hc * p.prefix_pairs + w.pair;
                 if (w.c < 0) {
-                    sg.part_row = (w.hc * w.ctx.pairs + w.pair + w.cta) * (2 * kTileRows);
+                    sg.part_row = (u + w.piece) * (2 * kTileRows);
                 } else {
-                    const int u = w.c * heads + w.hc;
-                    if (blk0 == 0) p.unit_start[u] = w.ub;
-                    sg.part_row = p.own_part_row + (u + w.cta) * p.gt;
+                    u = w.c * p.heads + w.hc;
+                    sg.part_row = p.own_part_row + (u + w.piece) * p.gt;
                     sg.part_rows = p.gt;
+                    u += p.heads * p.prefix_pairs;
                 }
-            } else if (blk0 == 0 && blk1 == nb) {
+                if (first && w.records) p.span[u] = Span{w.piece, last};
+            } else if (first && blk1 == nb) {
                 sg.part_row = -1;
             } else {
-                sg.part_row = (2 * w.cta + (blk0 == 0 ? 1 : 0)) * (2 * kTileRows);
-                if (blk0 == 0) {
-                    Split sp;
-                    sp.last = (w.ub + (nb - 1) * wt) / w.per;
-                    sp.tok0 = sg.tok0;
-                    sp.tok_end = sg.tok_end;
-                    sp.head0 = sg.head0;
-                    sp.nh = sg.nh;
-                    sp.mode = mode;
-                    p.split[w.cta] = sp;
-                }
+                const int slot = 2 * w.piece + (first ? 1 : 0);
+                sg.part_row = w.line == kFewLine ? p.few_part_row + slot * kFewTile : slot * (2 * kTileRows);
+                if (w.line == kFewLine) sg.part_rows = kFewTile;
+                if (first && w.records)
+                    p.split[w.line * p.pieces + w.piece] =
+                        Split{last, sg.tok0, sg.tok_end, sg.head0, sg.nh, mode, {0, 0}};
             }
         }
-        w.ub += nb * wt;
+        w.ub += static_cast<long long>(keys + kUnitCost) << two;
         w.x = w.ub;
         if (++w.pair == w.ctx.pairs) {
             w.pair = 0;
-            if (++w.hc == heads) {
+            if (++w.hc == p.heads) {
                 w.hc = 0;
-                while (w.x < w.x1 && w.c < p.B - 1) {
-                    w.ctx = load_ctx(p, ++w.c);
-                    if (w.ctx.head_cost != 0) break;
-                }
+                if (w.x < w.x1) w.c = next_ctx(w.c, w.line, w.ctx);
             }
         }
         if (some) return true;
     }
     return false;
-}
-
-// Where the partials of the output row (sequence b, query head h) are: row r1
-// of n1 tiles of kTileRows rows, 2 kTileRows apart from row1 on (the prefix),
-// and row r2 of n2 tiles of gt rows from row2 on (own keys).
-struct PrefixParts {
-    int n1, row1, r1;
-    int n2, row2, r2;
-};
-
-__host__ __device__ __forceinline__ PrefixParts prefix_parts(const PagedLine& p, int per,
-                                                             const Ctx& pre, const Ctx& own, int b,
-                                                             int hc, int hr) {
-    PrefixParts q = {0, 0, 0, 0, 0, 0};
-    if (pre.len > 0) {
-        const int tile = b / p.tpt;
-        const int pair = tile >> 1;
-        const int nb = unit_blocks(p, pre, pair);
-        const int ub = hc * pre.head_cost + pairs_cost(p, pre, pair);
-        const int i0 = ub / per;
-        q.n1 = (ub + (nb - 1) * mode_weight(p, unit_mode(pre, pair))) / per - i0 + 1;
-        q.row1 = (hc * pre.pairs + pair + i0) * (2 * kTileRows) + (tile & 1) * kTileRows;
-        q.r1 = (b - tile * p.tpt) * p.gt + hr;
-    }
-    if (own.len > 0) {
-        const int u = b * p.hkv * p.chunks + hc;
-        const int nb = unit_blocks(p, own, 0);
-        const int ub = p.unit_start[u];
-        const int i0 = ub / per;
-        q.n2 = (ub + (nb - 1) * mode_weight(p, own.last_mode)) / per - i0 + 1;
-        q.row2 = p.own_part_row + (u + i0) * p.gt;
-        q.r2 = hr;
-    }
-    return q;
 }
 
 // Row tiles of the query heads and tokens.
@@ -291,37 +301,31 @@ inline void set_tiles(PagedLine& p, int few_rows) {
     p.chunks = (p.group + kTileRows - 1) / kTileRows;
     p.gt = (p.group + p.chunks - 1) / p.chunks;
     p.tpt = kTileRows / p.gt;
+    p.heads = p.hkv * p.chunks;
     p.few_rows = few_rows;
-    p.w_two = 2;
-    p.w_one = 1;
-    p.w_few = 1;
-    p.min_per = 2;
+    p.prefix_pairs = ((p.B + p.tpt - 1) / p.tpt + 1) / 2;
 }
 
-// Partial rows and record bytes of a launch of `grid` CTAs; false if the line
-// or the rows could pass 32 bits.  Going along the line, each piece starts a
-// new unit, a new CTA or both, so unit + CTA numbers the pieces; ragged, only
-// a CTA's first and last piece are partial.
+// Partial rows and record bytes of a launch of `grid` CTAs; false if the rows
+// could pass 32 bits.  Going along a line, each segment starts a new unit, a
+// new piece or both, so unit + piece numbers them; ragged, only a piece's first
+// and last segment are partial.
 inline bool set_parts(PagedLine& p, int grid, long long& rows, long long& records) {
-    const long long heads = static_cast<long long>(p.hkv) * p.chunks;
-    const long long nb =
-        ((static_cast<long long>(p.max_pages) << p.page_shift) + kBlockKeys - 1) / kBlockKeys;
-    const long long pairs = (static_cast<long long>(p.num_tokens) + 2 * p.tpt - 1) / (2 * p.tpt);
-    long long line, own = 0;
+    p.pieces = grid;
+    const long long heads = p.heads;
+    long long own = 0, few = 0;
     if (p.prefix_mode) {
-        const long long nbp =
-            ((static_cast<long long>(p.max_prefix_pages) << p.page_shift) + kBlockKeys - 1) / kBlockKeys;
-        line = heads * (pairs * nbp + p.B * nb) * p.w_two;
-        own = (heads * pairs + grid) * 2 * kTileRows;
+        own = (heads * p.prefix_pairs + grid) * 2 * kTileRows;
         rows = own + (heads * p.B + grid) * p.gt;
-        records = heads * p.B * static_cast<long long>(sizeof(int));
+        records = heads * (p.prefix_pairs + p.B) * static_cast<long long>(sizeof(Span));
     } else {
-        line = heads * (pairs + p.B) * nb * p.w_two;
-        rows = 2LL * grid * 2 * kTileRows;
-        records = grid * static_cast<long long>(sizeof(Split));
+        few = 2LL * grid * 2 * kTileRows;
+        rows = few + 2LL * grid * kFewTile;
+        records = 2 * grid * static_cast<long long>(sizeof(Split));
     }
-    if (line > 0x7fffffffLL - 4096 || rows > 0x7fffffffLL) return false;
+    if (rows > 0x7fffffffLL || heads * (p.prefix_pairs + static_cast<long long>(p.B)) > 0x7fffffffLL) return false;
     p.own_part_row = static_cast<int>(own);
+    p.few_part_row = static_cast<int>(few);
     return true;
 }
 

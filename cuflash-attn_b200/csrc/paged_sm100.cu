@@ -218,7 +218,14 @@ __device__ sm100::StatusWord g_paged_status;
 constexpr int kTcThreads = 384;
 constexpr int kSegRing = 4;
 constexpr float kRescale = 8.0f;  // log2 units
-constexpr int kFewRows = 16;      // N of the transposed products
+constexpr int kFewRows = kFewTile;  // N of the transposed products
+
+// Where a CTA's piece of a line starts.
+struct Start {
+    Ctx ctx;
+    long long base, x0, x1, per;  // line position of the context; the piece; its length
+    int c;                        // the context, -2: no piece
+};
 
 template <int D>
 struct PagedGeom {
@@ -250,7 +257,7 @@ struct PagedGeom {
     static constexpr int kOffMl = kOffRing + kSlots * kTileBytes + kPad;
     static constexpr int kOffSeg = kOffMl + kTileRows * 8;
     static constexpr int kOffScan = kOffSeg + kSegRing * static_cast<int>(sizeof(Seg));
-    static constexpr int kOffBar = kOffScan + 96;  // 12 warp sums, start context
+    static constexpr int kOffBar = kOffScan + 192 + 2 * static_cast<int>(sizeof(Start));
     static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 5 * 2 + 2 + 2 * kSegRing + 1;
     static constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;
     static_assert(kOffBar % 8 == 0 && kSmemBytes <= 232448, "shared memory layout");
@@ -372,20 +379,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (cta_skip(&g_paged_status)) return;
 
-    // ---- this thread's contexts (first: their loads are the longest latency)
-    const int c_lo = ln.prefix_mode ? -1 : 0;
-    const int n_ctx = ln.B - c_lo;
-    const int heads = ln.hkv * ln.chunks;
-    const int run = (n_ctx + kTcThreads - 1) / kTcThreads;  // contexts per thread
-    const int c_first = c_lo + min(static_cast<int>(threadIdx.x) * run, n_ctx);
-    const int c_last = min(c_first + run, ln.B);
-    Ctx ctx1 = {};
-    int mine = 0;
-    for (int c = c_first; c < c_last; ++c) {
-        ctx1 = load_ctx(ln, c);
-        mine += ctx1.head_cost * heads;
-    }
-
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     uint8_t* sptr = smem_raw + (sbase - raw);
@@ -406,10 +399,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Seg* segs = reinterpret_cast<Seg*>(sptr + G::kOffSeg);
-    int* scan = reinterpret_cast<int*>(sptr + G::kOffScan);  // [12] warp sums
-    int* start_c = scan + 12;     // context the piece starts in, -2: none
-    int* start_base = scan + 13;  // its line position
-    Ctx* start_ctx = reinterpret_cast<Ctx*>(scan + 14);
+    long long* scan = reinterpret_cast<long long*>(sptr + G::kOffScan);  // [2 lines][12 warps]
+    Start* start = reinterpret_cast<Start*>(scan + 24);                   // [2 lines]
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -436,8 +427,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
-        *start_c = -2;
-        if (!ln.prefix_mode) ln.split[blockIdx.x].last = -1;
+        if (!ln.prefix_mode) ln.split[blockIdx.x].last = ln.split[gridDim.x + blockIdx.x].last = -1;
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
         prefetch_tmap(&tmQ);
@@ -449,42 +439,67 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_relinquish();
     }
 
-    // ---- the line: contexts' lengths summed over the block
-    int incl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
-    }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kTcThreads / 32; ++w) {
-        const int v = scan[w];
-        if (w < warp) before += v;
-        total += v;
-    }
-    const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), ln.min_per);
-    const int x0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
-    const int x1 = min(x0 + per, total);
-    {
-        int base = before + incl - mine;
-        if (x0 < x1 && x0 >= base && x0 < base + mine) {
-            for (int c = c_first; c < c_last; ++c) {
-                if (run > 1) ctx1 = load_ctx(ln, c);
-                const int cost = ctx1.head_cost * heads;
-                if (x0 < base + cost) {
-                    *start_c = c;
-                    *start_base = base;
-                    *start_ctx = ctx1;
-                    break;
+    // ---- the lines: contexts' lengths summed over the block, then the context
+    // each of this CTA's pieces starts in
+    const int c_lo = ln.prefix_mode ? -1 : 0;
+    const int n_cta = static_cast<int>(gridDim.x);
+    const int run = (ln.B - c_lo + kTcThreads - 1) / kTcThreads;  // contexts per thread
+    const int c_first = c_lo + static_cast<int>(threadIdx.x) * run;
+    long long mine[2] = {0, 0};  // pass 0: lengths; pass 1: position behind the contexts so far
+    Ctx ctx = {};
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+        for (int c = c_first; c < min(c_first + run, ln.B); ++c) {
+            if (pass == 0 || run > 1) ctx = load_ctx(ln, c);
+            const int l = line_of(ctx);
+            const long long cost = ctx.head_cost * ln.heads;
+            long long& at = l == kTiles ? mine[0] : mine[1];
+            if (pass == 1) {
+                Start& st = start[l];
+                if (st.x0 < st.x1 && st.x0 >= at && st.x0 < at + cost) {
+                    st.ctx = ctx;
+                    st.base = at;
+                    st.c = c;
                 }
-                base += cost;
             }
+            at += cost;
         }
+        if (pass == 1) break;
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+            long long incl = mine[l];
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += v;
+            }
+            if (lane == 31) scan[l * 12 + warp] = incl;
+            mine[l] = incl - mine[l];
+        }
+        __syncthreads();
+        long long sum[2] = {0, 0};
+#pragma unroll 1
+        for (int w = 0; w < kTcThreads / 32; ++w) {
+            if (w == warp) {
+                mine[0] += sum[0];
+                mine[1] += sum[1];
+            }
+            sum[0] += scan[w];
+            sum[1] += scan[12 + w];
+        }
+        if (threadIdx.x < 2) {
+            const long long line = threadIdx.x == kTiles ? sum[0] : sum[1];
+            const int piece = threadIdx.x == kTiles ? static_cast<int>(blockIdx.x)
+                                                    : n_cta - 1 - static_cast<int>(blockIdx.x);
+            Start& st = start[threadIdx.x];
+            st.c = -2;
+            st.per = piece_length(line, n_cta);
+            st.x0 = min(piece * st.per, line);
+            st.x1 = min(st.x0 + st.per, line);
+        }
+        __syncthreads();
     }
-    if (threadIdx.x == 0 && blockIdx.x == 0) *ln.per = per;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -498,6 +513,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t since = tick();
     auto poll = [&](uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
         while (!mbar_try_wait(addr, parity))
             if (*abort_flag || tick() - since > kWaitTicks) return false;
         return true;
@@ -506,6 +522,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // from the softmax warps of its quarter.
     auto poll_idle = [&](uint64_t* bar, uint32_t parity, unsigned ns) -> bool {
         const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
         while (!mbar_try_wait(addr, parity)) {
             if (*abort_flag || tick() - since > kWaitTicks) return false;
             __nanosleep(ns);
@@ -538,6 +555,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             };
             int entry_next_seg = 0;
             bool have_next = false;
+#pragma unroll 1
             for (int k = 0;; ++k) {
                 ok = poll(seg_full + k % kSegRing, (k / kSegRing) & 1);
                 ok = __all_sync(0xffffffffu, ok);
@@ -556,6 +574,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const bool few = sg.mode == kFew;
                     const uint32_t bytes =
                         static_cast<uint32_t>(ln.gt * (few ? p.few_tok : ln.tpt)) * G::kRowBytes;
+#pragma unroll 1
                     for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
                         const int slot = sg.mode == kTwoTiles ? u : qs;
                         if (q_cnt[slot] > 0)
@@ -570,6 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 if (sg.mode != kTwoTiles) qs ^= 1;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
+#pragma unroll 1
                 for (int j = 0; ok && j < sg.n_blk; ++j) {
                     const int blk = sg.blk0 + j;
                     if (blk * boxes / 32 != chunk) {
@@ -631,8 +651,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // product takes is then warp-uniform for the compiler (registers of
             // the uniform datapath, no per-thread copies before each instruction).
             // What it spends between products is on every step's critical path,
-            // so the steps are unrolled over the two streams, ring positions are
-            // counted up, and a step waiting for its O is one word of flags.
+            // so ring positions are counted up and a step waiting for its O is a
+            // word of flags.
             {
                 const uint32_t leader = elect_lane();
                 const uint32_t tm = uniform(tmem);
@@ -649,8 +669,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                    kFreeQ = 64, kQSlot1 = 128;
                 uint32_t ks = 0, kph = 0;  // ring slot and phase of the next block's K
                 uint32_t vs = 1, vph = 0;  // of the V of the step whose O is next
-                uint32_t due0 = 0, due1 = 0;  // each stream's step that has its S but not its O
-                uint32_t par0 = 0, par1 = 0;  // phases of bar_p
+                uint32_t due = 0;  // 16 bits per stream: its step that has its S but not its O
+                uint32_t par = 0;  // bit t: phase of bar_p[t]
                 uint32_t qph = 0;             // bit u: phase of bar_q[u]
                 int k = 0, qs = 0, cur_q = 0;
                 int i = 0, steps = 0, mode = kTwoTiles;
@@ -663,8 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 };
                 // S of the next step (stream t); its flags, 0 at the end
-                auto issue_s = [&](auto stream) -> uint32_t {
-                    constexpr int t = decltype(stream)::value;
+                auto issue_s = [&](int t) -> uint32_t {
                     if (i == steps) {
                         if (!wait(seg_full + k % kSegRing, (k / kSegRing) & 1)) return 0;
                         const Seg& sg = segs[k % kSegRing];
@@ -724,13 +743,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     return flags;
                 };
                 // O of stream t's step, in step order
-                auto issue_o = [&](auto stream, uint32_t flags) -> bool {
-                    constexpr int t = decltype(stream)::value;
-                    uint32_t& par = t ? par1 : par0;
+                auto issue_o = [&](int t, uint32_t flags) -> bool {
+                    const uint32_t phase = (par >> t) & 1;
                     if ((flags & kWaitV) && !wait(full + vs, vph)) return false;
-                    if (!wait(bar_p + t, par)) return false;
+                    if (!wait(bar_p + t, phase)) return false;
                     const uint64_t v0 = pg_vdesc<D>(sb + G::kOffRing + vs * G::kTileBytes);
-                    constexpr int kO = 256 + t * 128;
+                    const uint32_t o_tm = tm + 256 + t * 128;
                     const uint32_t acc = (flags & kAcc) ? 1u : 0u;
                     tc_fence_after();
                     if (G::kHasFew && (flags & kIsFew)) {
@@ -739,26 +757,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                      kLayoutSw128);
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ss(leader, tm + kO, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
+                            mma_ss(leader, o_tm, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
                                        kk > 0 ? 1u : acc);
                         if (flags & kFreeQ) commit(leader, bar_qfree + ((flags & kQSlot1) ? 1 : 0));
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_ts(leader, tm + kO, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
+                            mma_ts(leader, o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
                                        kk > 0 ? 1u : acc);
-                        if (!wait(bar_p2 + t, par)) return false;
+                        if (!wait(bar_p2 + t, phase)) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk)
-                            mma_ts(leader, tm + kO, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
+                            mma_ts(leader, o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
                     }
                     if (flags & kLast) commit(leader, bar_o + t);
                     if (flags & kFreeV) {
                         commit(leader, empty + vs);
                         next_slot(vs, vph);
                     }
-                    par ^= 1;
+                    par ^= 1u << t;
                     return true;
                 };
                 // Stream t's turn: its O, then its next S behind it (in order, so
@@ -766,21 +784,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // other stream's O does not wait behind an S whose keys have not
                 // landed; and the segment's products end before the next segment
                 // begins, which may need the query slot that holds P^T.
-                auto turn = [&](auto stream, uint32_t& due, uint32_t& other) -> bool {
-                    constexpr int t = decltype(stream)::value;
-                    std::integral_constant<int, t ^ 1> next;
-                    if (due != 0 && !issue_o(stream, due)) return false;
-                    due = 0;
+#pragma unroll 1
+                for (int t = 0;; t ^= 1) {
+                    const uint32_t mine = (due >> (16 * t)) & 0xffffu;
+                    if (mine != 0 && !issue_o(t, mine)) break;
+                    uint32_t other = (due >> (16 * (t ^ 1))) & 0xffffu;
                     if (G::kHasFew && mode == kFew && other != 0 &&
                         (i == steps || !__all_sync(0xffffffffu, mbar_test(full + ks, kph)))) {
-                        if (!issue_o(next, other)) return false;
+                        if (!issue_o(t ^ 1, other)) break;
                         other = 0;
                     }
-                    if (!end) due = issue_s(stream);
-                    return ok;
-                };
-                while (turn(std::integral_constant<int, 0>(), due0, due1) &&
-                       turn(std::integral_constant<int, 1>(), due1, due0) && (due0 | due1) != 0) {
+                    const uint32_t next = end ? 0 : issue_s(t);
+                    due = (next << (16 * t)) | (other << (16 * (t ^ 1)));
+                    if (!ok || due == 0) break;
                 }
                 // all products (and their commits) retire before teardown
                 commit(leader, bar_done);
@@ -790,26 +806,57 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
         } else if (warp == 2) {
             // ------------------------------------------------ units and segments
-            if (lane == 0) {
-                int k = 0;
-                auto emit = [&](const Seg& sg) {
-                    if (k >= kSegRing)
-                        ok = poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500);
-                    if (!ok) return;
-                    since = tick();
+            // The warp walks converged; lane 0 writes.  CTAs that share a TPC's
+            // instruction cache go through the lines in the same order, their
+            // neighbours in the other one.
+            unsigned smid;
+            asm volatile("mov.u32 %0, %%smid;" : "=r"(smid));
+            int k = 0;
+            auto emit = [&](const Seg& sg) {
+                if (k >= kSegRing)
+                    ok = __all_sync(0xffffffffu,
+                                    poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500));
+                if (!ok) return;
+                since = tick();
+                if (lane == 0) {
                     segs[k % kSegRing] = sg;
                     mbar_arrive(seg_full + k % kSegRing);
-                    ++k;
-                };
-                Seg sg = {};
-                if (x0 < x1 && *start_c >= c_lo) {
-                    Walk w;
-                    walk_start(ln, w, *start_ctx, *start_c, *start_base, x0, x1, per, blockIdx.x);
-                    while (ok && walk_next(ln, w, sg)) emit(sg);
                 }
-                sg.n_blk = 0;
-                if (ok) emit(sg);
+                ++k;
+            };
+            // 32 contexts at a time: a batch may have many between two of a line
+            auto next_ctx = [&](int c, int line, Ctx& out) -> int {
+#pragma unroll 1
+                for (int base = c + 1; base < ln.B; base += 32) {
+                    Ctx x = {};
+                    if (base + lane < ln.B) x = load_ctx(ln, base + lane);
+                    const unsigned hit = __ballot_sync(0xffffffffu, x.head_cost != 0 && line_of(x) == line);
+                    if (hit == 0) continue;
+                    const int src = __ffs(hit) - 1;
+                    out.tok = __shfl_sync(0xffffffffu, x.tok, src);
+                    out.ntok = __shfl_sync(0xffffffffu, x.ntok, src);
+                    out.len = __shfl_sync(0xffffffffu, x.len, src);
+                    out.pairs = __shfl_sync(0xffffffffu, x.pairs, src);
+                    out.last_mode = __shfl_sync(0xffffffffu, x.last_mode, src);
+                    out.head_cost = __shfl_sync(0xffffffffu, x.head_cost, src);
+                    return base + src;
+                }
+                return c;  // not reached while the walk is inside the line
+            };
+            Seg sg = {};
+#pragma unroll 1
+            for (int turn = 0; turn < 2 && ok; ++turn) {
+                const int l = (turn ^ static_cast<int>(smid >> 1)) & 1;
+                if (start[l].c < c_lo) continue;
+                Walk w;
+                walk_start(ln, w, start[l].ctx, start[l].c, start[l].base, start[l].x0, start[l].x1, start[l].per, l,
+                           l == kTiles ? static_cast<int>(blockIdx.x) : n_cta - 1 - static_cast<int>(blockIdx.x),
+                           lane == 0);
+#pragma unroll 1
+                while (ok && walk_next(ln, w, sg, next_ctx)) emit(sg);
             }
+            sg.n_blk = 0;
+            if (ok) emit(sg);
             __syncwarp();
         }
     } else {
@@ -873,6 +920,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 neg_m[g] = 0.f;
                 l_part[g] = 0.f;
             }
+#pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 if (!wait(bar_s + t, s_cnt & 1)) return;
                 ++s_cnt;
@@ -1014,8 +1062,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     l = w0 * l + w1 * l1;
                     o = w0 * o + w1 * __uint_as_float(ov2[g]);
                 }
-                o *= l > 0.f ? 1.f / l : 0.f;
-                const float lse2 = l > 0.f ? M + log2f(l) : -INFINITY;
+                o *= l > 0.f ? __fdividef(1.f, l) : 0.f;
+                const float lse2 = l > 0.f ? M + __log2f(l) : -INFINITY;
                 if (g < ncol && h < sg.nh && r < D) {  // lane r holds column r of the head
                     if (sg.part_row >= 0) {
                         p.O_part[static_cast<long long>(sg.part_row) * D + ((r >> 2) * sg.part_rows + g) * 4 +
@@ -1038,6 +1086,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         };
         int blocks = 0;  // of the last segment
+#pragma unroll 1
         for (int k = 0; ok; ++k) {
             if (!wait(seg_full + k % kSegRing, (k / kSegRing) & 1)) break;
             const Seg sg = segs[k % kSegRing];
@@ -1072,6 +1121,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row_end = ln.causal ? min(sg.len - 1, tile_lim + tok_r) : sg.len - 1;
 
             float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 if (!wait(bar_s + t, s_cnt & 1)) break;
                 ++s_cnt;
@@ -1124,7 +1174,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 // S_t of this step was issued behind O_t of the last one, so O_t is at rest
                 if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
+#pragma unroll 1
                     for (int cb = 0; cb < D / 16; ++cb) {
                         uint32_t o[16];
                         tmem_ld_x16(o_tmem + cb * 16, o);
@@ -1190,14 +1240,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 l_run = w0 * l_run + w1 * o2.y;
                 m_run = M;
             }
-            const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;
+            const float inv_l = l_run > 0.f ? __fdividef(1.f, l_run) : 0.f;
             w0 *= inv_l;
             w1 *= inv_l;
-            const float lse2 = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
+            const float lse2 = l_run > 0.f ? m_run + __log2f(l_run) : -INFINITY;
             if (active) {
                 const long long prow = static_cast<long long>(sg.part_row) + tile * kTileRows;
                 const long long orow = static_cast<long long>(token) * ln.hq + sg.head0 + head_r;
-#pragma unroll
+#pragma unroll 1
                 for (int cb = 0; cb < D / 32; ++cb) {
                     uint32_t o[32];
                     tmem_ld_x32(o_tmem + cb * 32, o);
@@ -1263,92 +1313,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // the line.  A block takes 32 rows (one per lane, so that loads of the
 // partials' layout are contiguous); its 8 warps share the columns, four at a
 // time, and the result is transposed through shared memory for its stores.
-// Bound by latency (two dependent rounds of loads), not bytes.
+// Bound by latency (dependent rounds of loads, instruction fetches), not bytes.
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
 
-template <int D>
-struct JoinAcc {
-    static constexpr int kQuads = D / 4 / (kJoinThreads / 32);  // per warp
-    float4 v[kQuads];
-    float tot;
+// A lane's partials: n of them, tiles of `rows` rows `step` rows apart from
+// `base` on, row r of each.
+struct Parts {
+    int n, base, step, rows, r;
 };
 
-// Adds n partials: row r of the tiles of `rows` rows at base, base + step, ...
-template <int D>
-__device__ __forceinline__ void join_add(const TcParams& p, JoinAcc<D>& a, float M, int n, int base,
-                                         int step, int rows, int r) {
-    constexpr int Q = JoinAcc<D>::kQuads;
-    constexpr int kFlight = 16 / Q;  // partials in flight: 16 loads of 16 bytes per thread
-    for (int k0 = 0; k0 < n; k0 += kFlight) {
-        float4 s[kFlight][Q];
+// Joins the partials of both lists for this block's 32 rows and writes them;
+// lane's row goes to out_row (-1: none).
+template <typename T, int D>
+__device__ __forceinline__ void join_rows(const TcParams& p, const Parts& a, const Parts& b, int out_row) {
+    constexpr int Q = D / 4 / (kJoinThreads / 32);  // column quads per warp
+    constexpr int kFlight = 16 / Q;                 // partials in flight: 16 loads of 16 bytes
+    constexpr int kPitch = D + 8;  // 16-bit elements; rows 16 bytes apart in the banks
+    __shared__ __align__(16) T tile[32][kPitch];
+    __shared__ int out[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = a.n + b.n;
+    auto tile_row = [&](int k) -> int { return k < a.n ? a.base + k * a.step : b.base + (k - a.n) * b.step; };
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[tile_row(k) + (k < a.n ? a.r : b.r)]);
+    float4 acc[Q];
+    float tot = 0.f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < n && M != -INFINITY; k0 += kFlight) {
+        float4 v[kFlight][Q];
         float w[kFlight];
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-            const int at = base + min(k0 + k, n - 1) * step;
+            const int kk = min(k0 + k, n - 1);
+            const int at = tile_row(kk), r = kk < a.n ? a.r : b.r, rows = kk < a.n ? a.rows : b.rows;
             w[k] = p.L_part[at + r];
             const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(at) * D) + r +
-                                (threadIdx.x >> 5) * Q * rows;
+                                warp * Q * rows;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) s[k][q] = src[q * rows];
+            for (int q = 0; q < Q; ++q) v[k][q] = src[q * rows];
         }
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
             const float wk = k0 + k < n ? sm100::ex2_approx(w[k] - M) : 0.f;
-            a.tot += wk;
+            tot += wk;
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                a.v[q].x = fmaf(wk, s[k][q].x, a.v[q].x);
-                a.v[q].y = fmaf(wk, s[k][q].y, a.v[q].y);
-                a.v[q].z = fmaf(wk, s[k][q].z, a.v[q].z);
-                a.v[q].w = fmaf(wk, s[k][q].w, a.v[q].w);
+                acc[q].x = fmaf(wk, v[k][q].x, acc[q].x);
+                acc[q].y = fmaf(wk, v[k][q].y, acc[q].y);
+                acc[q].z = fmaf(wk, v[k][q].z, acc[q].z);
+                acc[q].w = fmaf(wk, v[k][q].w, acc[q].w);
             }
         }
     }
-}
-
-// Largest log2-sum-exp of n partials (same rows as join_add).
-__device__ __forceinline__ float join_max(const TcParams& p, float M, int n, int base, int step, int r) {
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[base + k * step + r]);
-    return M;
-}
-
-// Writes this block's 32 rows; lane's row goes to out_row (-1: none).
-template <typename T, int D>
-__device__ __forceinline__ void join_store(const TcParams& p, const JoinAcc<D>& a, float M, int out_row) {
-    constexpr int kPitch = D + 8;  // 16-bit elements; rows 16 bytes apart in the banks
-    __shared__ __align__(16) T tile[32][kPitch];
-    __shared__ int rows[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float inv = a.tot > 0.f ? 1.f / a.tot : 0.f;
+    const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
 #pragma unroll
-    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) {
+    for (int q = 0; q < Q; ++q) {
         uint2 v;
-        v.x = DType<T>::pack2(a.v[q].x * inv, a.v[q].y * inv);
-        v.y = DType<T>::pack2(a.v[q].z * inv, a.v[q].w * inv);
-        *reinterpret_cast<uint2*>(&tile[lane][(warp * JoinAcc<D>::kQuads + q) * 4]) = v;
+        v.x = DType<T>::pack2(acc[q].x * inv, acc[q].y * inv);
+        v.y = DType<T>::pack2(acc[q].z * inv, acc[q].w * inv);
+        *reinterpret_cast<uint2*>(&tile[lane][(warp * Q + q) * 4]) = v;
     }
     if (warp == 0) {
-        rows[lane] = out_row;
-        if (out_row >= 0) p.L[out_row] = a.tot > 0.f ? (M + log2f(a.tot)) * kLn2 : -INFINITY;
+        out[lane] = out_row;
+        if (out_row >= 0) p.L[out_row] = tot > 0.f ? (M + __log2f(tot)) * kLn2 : -INFINITY;
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = threadIdx.x; e < 32 * (D / 8); e += kJoinThreads) {
-        const int r = e / (D / 8), c = e - r * (D / 8);
-        if (rows[r] >= 0)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(rows[r]) * D + c * 8) =
+        const int r = e / (D / 8), c = e % (D / 8);
+        if (out[r] >= 0)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(out[r]) * D + c * 8) =
                 *reinterpret_cast<const uint4*>(&tile[r][c * 8]);
     }
-}
-
-template <int D>
-__device__ __forceinline__ JoinAcc<D> join_zero() {
-    JoinAcc<D> a;
-#pragma unroll
-    for (int q = 0; q < JoinAcc<D>::kQuads; ++q) a.v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-    a.tot = 0.f;
-    return a;
 }
 
 __device__ __forceinline__ bool partials_ready() {
@@ -1361,69 +1401,70 @@ __device__ __forceinline__ bool partials_ready() {
 // then the sequence's own.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-    paged_join_prefix_kernel(const __grid_constant__ TcParams p, int groups) {
+    paged_join_prefix_kernel(const __grid_constant__ TcParams p) {
     const PagedLine& ln = p.ln;
-    const int hc = blockIdx.x / groups;
-    const int row = (blockIdx.x - hc * groups) * 32 + (threadIdx.x & 31);  // of the head chunk
+    const int hc = blockIdx.y;
+    const int row = blockIdx.x * 32 + (threadIdx.x & 31);  // of the head chunk
     const int tile = row / kTileRows;
-    const int r = row - tile * kTileRows;
+    const int r = row % kTileRows;
     const int tok_r = r / ln.gt;
     const int hr = r - tok_r * ln.gt;
     const int b = tile * ln.tpt + tok_r;
-    const int hk = hc / ln.chunks, ch = hc - hk * ln.chunks;
-    const bool valid = tok_r < ln.tpt && b < ln.B && ch * ln.gt + hr < ln.group;
-    const Ctx pre = load_ctx(ln, -1);
-    const Ctx own = load_ctx(ln, valid ? b : 0);
+    const int hk = ln.chunks == 1 ? hc : hc / ln.chunks;
+    const int head = hk * ln.group + (hc - hk * ln.chunks) * ln.gt + hr;
+    const bool valid = tok_r < ln.tpt && b < ln.B && head < (hk + 1) * ln.group;
+    const bool has_own = valid && ln.seq_lens[b] > 0;
+    const bool has_prefix = valid && *ln.prefix_len > 0;
     if (!partials_ready()) return;
-    PrefixParts q = {};
-    if (valid) q = prefix_parts(ln, *ln.per, pre, own, b, hc, hr);
-    float M = join_max(p, -INFINITY, q.n1, q.row1, 2 * kTileRows, q.r1);
-    M = join_max(p, M, q.n2, q.row2, ln.gt, q.r2);
-    JoinAcc<D> a = join_zero<D>();
-    if (M != -INFINITY) {
-        join_add<D>(p, a, M, q.n1, q.row1, 2 * kTileRows, kTileRows, q.r1);
-        join_add<D>(p, a, M, q.n2, q.row2, ln.gt, ln.gt, q.r2);
+    Parts pre = {}, own = {};
+    if (has_prefix) {
+        const int u = hc * ln.prefix_pairs + (tile >> 1);
+        const Span sp = ln.span[u];
+        pre = Parts{sp.last - sp.first + 1, (u + sp.first) * (2 * kTileRows) + (tile & 1) * kTileRows,
+                    2 * kTileRows, kTileRows, r};
     }
-    join_store<T, D>(p, a, M, valid ? b * ln.hq + hk * ln.group + ch * ln.gt + hr : -1);
+    if (has_own) {
+        const int u = b * ln.heads + hc;
+        const Span sp = ln.span[ln.heads * ln.prefix_pairs + u];
+        own = Parts{sp.last - sp.first + 1, ln.own_part_row + (u + sp.first) * ln.gt, ln.gt, ln.gt, hr};
+    }
+    join_rows<T, D>(p, pre, own, valid ? b * ln.hq + head : -1);
 }
 
-// Block (i, y): rows [32 y, 32 y + 32) of the unit whose first blocks CTA i
-// had and whose last CTA split[i].last had.
+// Block (i, y): rows [32 y, 32 y + 32) of the row tiles (y < 8), or the few
+// rows (y = 8), of the unit that piece i of the line had the first blocks of
+// and piece split.last the last.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-    paged_join_split_kernel(const __grid_constant__ TcParams p, int) {
+    paged_join_split_kernel(const __grid_constant__ TcParams p) {
     const PagedLine& ln = p.ln;
     if (!partials_ready()) return;
     const int i = static_cast<int>(blockIdx.x);
-    const Split sp = ln.split[i];
+    const bool few = blockIdx.y == 2 * kTileRows / 32;
+    const Split sp = ln.split[(few ? ln.pieces : 0) + i];
     if (sp.last <= i) return;
-    const int row = blockIdx.y * 32 + (threadIdx.x & 31);
+    const int row = (few ? 0 : blockIdx.y * 32) + (threadIdx.x & 31);
     const int tile = row / kTileRows;
-    const int r = row - tile * kTileRows;
+    const int r = row % kTileRows;
     if (tile == 1 && sp.mode != kTwoTiles) return;
     const int tok_r = r / ln.gt;
     const int hr = r - tok_r * ln.gt;
     const int token = sp.tok0 + tile * ln.tpt + tok_r;
     const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
     if (__syncthreads_or(valid) == 0) return;
-    const int n = valid ? sp.last - i + 1 : 0;
-    // CTA i's last piece, then the first ones of the CTAs behind it
-    const int base0 = (2 * i + 1) * (2 * kTileRows) + tile * kTileRows;
-    const int base1 = (2 * i + 2) * (2 * kTileRows) + tile * kTileRows;
-    float M = join_max(p, -INFINITY, min(n, 1), base0, 0, r);
-    M = join_max(p, M, n - 1, base1, 4 * kTileRows, r);
-    JoinAcc<D> a = join_zero<D>();
-    if (M != -INFINITY) {
-        join_add<D>(p, a, M, min(n, 1), base0, 0, kTileRows, r);
-        join_add<D>(p, a, M, n - 1, base1, 4 * kTileRows, kTileRows, r);
-    }
-    join_store<T, D>(p, a, M, valid ? token * ln.hq + sp.head0 + hr : -1);
+    // piece i's last segment, then the first ones of the pieces behind it
+    const int rows = few ? kFewTile : kTileRows;      // of a tile
+    const int slot = few ? kFewTile : 2 * kTileRows;  // of a segment
+    const int base = (few ? ln.few_part_row : tile * kTileRows) + 2 * i * slot;
+    const Parts head = {valid ? 1 : 0, base + slot, 0, rows, r};
+    const Parts rest = {valid ? sp.last - i : 0, base + 2 * slot, 2 * slot, rows, r};
+    join_rows<T, D>(p, head, rest, valid ? token * ln.hq + sp.head0 + hr : -1);
 }
 
 // Launches `kern` so that its blocks may be scheduled while the kernel before
 // it on the stream still runs (they wait for it inside).
-cudaError_t launch_behind(void (*kern)(const TcParams, int), dim3 grid, cudaStream_t stream,
-                          const TcParams& p, int arg) {
+cudaError_t launch_behind(void (*kern)(const TcParams), dim3 grid, cudaStream_t stream,
+                          const TcParams& p) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kJoinThreads);
@@ -1433,7 +1474,7 @@ cudaError_t launch_behind(void (*kern)(const TcParams, int), dim3 grid, cudaStre
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p, arg);
+    return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -1495,8 +1536,8 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), G::kSmemBytes))
         return FlashAttentionError::CUDA_ERROR;
 
-    // workspace: piece length, unit starts or split records, partial rows
-    const size_t off_rec = 256;
+    // workspace: records of the units' pieces, partial rows
+    const size_t off_rec = 0;
     const size_t off_l = off_rec + align256(static_cast<size_t>(records));
     const size_t off_o = off_l + align256(static_cast<size_t>(rows) * sizeof(float));
     const size_t bytes = off_o + static_cast<size_t>(rows) * D * sizeof(float);
@@ -1504,8 +1545,7 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     const FlashAttentionError werr = workspace_alloc(&ws, bytes, stream);
     if (werr != FlashAttentionError::SUCCESS) return werr;
     char* base = static_cast<char*>(ws);
-    ln.per = reinterpret_cast<int*>(base);
-    ln.unit_start = reinterpret_cast<int*>(base + off_rec);
+    ln.span = reinterpret_cast<Span*>(base + off_rec);
     ln.split = reinterpret_cast<Split*>(base + off_rec);
     p.L_part = reinterpret_cast<float*>(base + off_l);
     p.O_part = reinterpret_cast<float*>(base + off_o);
@@ -1515,13 +1555,13 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) {
         if (ln.prefix_mode) {
-            const long long tiles = (ln.B + ln.tpt - 1) / ln.tpt;
-            const long long last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
-            const int groups = static_cast<int>((tiles - 1) * (kTileRows / 32) + (last + 31) / 32);
-            err = launch_behind(paged_join_prefix_kernel<T, D>,
-                                dim3(static_cast<unsigned>(ln.hkv * ln.chunks * groups)), stream, p, groups);
+            const int tiles = (ln.B + ln.tpt - 1) / ln.tpt;
+            const int last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
+            const int groups = (tiles - 1) * (kTileRows / 32) + (last + 31) / 32;
+            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads), stream, p);
         } else {
-            err = launch_behind(paged_join_split_kernel<T, D>, dim3(grid, 2 * kTileRows / 32), stream, p, 0);
+            err = launch_behind(paged_join_split_kernel<T, D>,
+                                dim3(grid, 2 * kTileRows / 32 + (G::kHasFew ? 1 : 0)), stream, p);
         }
         if (err != cudaSuccess) cudaGetLastError();
     }

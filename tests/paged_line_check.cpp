@@ -29,13 +29,6 @@ int main(int argc, char** argv) {
     std::mt19937 gen(1);
     auto R = [&](int a, int b) { return static_cast<int>(a + gen() % static_cast<unsigned>(b - a + 1)); };
     int it = -1;
-    for (int n = 0; n <= 40; ++n)  // the closed form against the sum itself
-        for (int k = 0; k < 200; ++k) {
-            const int m = R(1, 200), a = R(0, 300), b = R(0, 5000);
-            int s = 0;
-            for (int i = 0; i < n; ++i) s += (a * i + b) / m;
-            CHECK(floor_sum(n, m, a, b) == s);
-        }
     long long pieces = 0;
     for (it = 0; it < rounds; ++it) {
         PagedLine p{};
@@ -61,53 +54,68 @@ int main(int argc, char** argv) {
         p.seq_lens = lens.data();
         p.cu_seqlens = cu.data();
         p.prefix_len = &plen;
-        set_tiles(p, R(0, 2) ? 16 : 0);
+        const int few[4] = {0, 4, 8, 16};
+        set_tiles(p, few[R(0, 3)]);
         CHECK(p.tpt >= 1 && p.tpt * p.gt <= kTileRows && p.gt * p.chunks >= group &&
               p.gt * (p.chunks - 1) < group);
         const int grid = R(0, 2) ? 148 : R(1, 200);
         long long rows, records;
         CHECK(set_parts(p, grid, rows, records));
-        int per;
-        std::vector<int> starts(static_cast<size_t>(p.B) * p.hkv * p.chunks, -1);
-        std::vector<Split> split(grid);
+        long long per[2];
+        std::vector<Span> span(static_cast<size_t>(p.B + p.prefix_pairs) * p.heads, Span{-1, -1});
+        std::vector<Split> split(2 * grid);
         for (auto& s : split) s.last = -1;
-        p.per = &per;
         if (p.prefix_mode)
-            p.unit_start = starts.data();
+            p.span = span.data();
         else
             p.split = split.data();
         const int c_lo = p.prefix_mode ? -1 : 0;
-        const int heads = p.hkv * p.chunks;
-        std::vector<int> base;
-        int total = 0;
+        const int heads = p.heads;
+        std::vector<long long> base;  // position of each context on its line
+        long long total[2] = {0, 0};
         for (int c = c_lo; c < p.B; ++c) {
             const Ctx x = load_ctx(p, c);
-            int sum = 0;
+            long long sum = 0;
             if (x.head_cost)
                 for (int q = 0; q < x.pairs; ++q) {
                     CHECK(pairs_cost(p, x, q) == sum);
-                    sum += unit_blocks(p, x, q) * mode_weight(p, unit_mode(x, q));
+                    sum += unit_length(p, x, q);
                 }
             CHECK(x.head_cost == sum);
-            base.push_back(total);
-            total += x.head_cost * heads;
+            base.push_back(total[line_of(x)]);
+            total[line_of(x)] += x.head_cost * heads;
         }
-        per = std::max((total + grid - 1) / grid, p.min_per);
+        auto next_ctx = [&](int c, int line, Ctx& out) {
+            while (++c < p.B) {
+                out = load_ctx(p, c);
+                if (out.head_cost != 0 && line_of(out) == line) return c;
+            }
+            CHECK(!"a context behind the last");
+            return c;
+        };
         using Key = std::tuple<int, int, int>;  // context, first head, first token
         std::map<Key, std::vector<std::pair<int, Seg>>> units;
         std::set<int> taken;
-        for (int i = 0; i < grid; ++i) {
-            const int x0 = i * per, x1 = std::min(x0 + per, total);
+        for (int li = 0; li < 2 * grid; ++li) {
+            const int line = li / grid, i = li % grid;
+            per[line] = piece_length(total[line], grid);
+            CHECK(per[line] * grid >= total[line]);
+            const long long x0 = i * per[line], x1 = std::min(x0 + per[line], total[line]);
             if (x0 >= x1) continue;
             int c = c_lo;
-            while (c + 1 < p.B && base[c + 1 - c_lo] <= x0) ++c;
-            while (load_ctx(p, c).head_cost == 0) --c;
+            while (true) {  // the context that holds x0
+                const Ctx x = load_ctx(p, c);
+                if (line_of(x) == line && x0 >= base[c - c_lo] && x0 < base[c - c_lo] + x.head_cost * heads) break;
+                ++c;
+                CHECK(c < p.B);
+            }
             Walk w;
-            walk_start(p, w, load_ctx(p, c), c, base[c - c_lo], x0, x1, per, i);
+            walk_start(p, w, load_ctx(p, c), c, base[c - c_lo], x0, x1, per[line], line, i, true);
             Seg s = {};
             int n = 0;
-            while (walk_next(p, w, s)) {
+            while (walk_next(p, w, s, next_ctx)) {
                 ++n;
+                CHECK((s.mode == kFew) == (line == kFewLine));
                 ++pieces;
                 CHECK(s.n_blk > 0 && s.blk0 >= 0);
                 CHECK(s.tok0 >= 0 && s.tok0 < s.tok_end && s.tok_end <= p.num_tokens);
@@ -118,14 +126,16 @@ int main(int argc, char** argv) {
                 if (s.mode == kFew) CHECK((s.tok_end - s.tok0) * p.gt <= p.few_rows);
                 if (s.part_row >= 0) {
                     const bool own = p.prefix_mode && s.ctx >= 0;
-                    const int span = own ? p.gt : 2 * kTileRows;
-                    CHECK(s.part_rows == (own ? p.gt : kTileRows));
-                    CHECK(s.part_row + span <= rows);
-                    for (int q = 0; q < span; q += own ? 1 : kTileRows) CHECK(taken.insert(s.part_row + q).second);
+                    const bool few = !p.prefix_mode && s.mode == kFew;
+                    const int span = own ? p.gt : (few ? kFewTile : 2 * kTileRows);
+                    CHECK(s.part_rows == (own ? p.gt : (few ? kFewTile : kTileRows)));
+                    CHECK(s.mode != kFew || (s.tok_end - s.tok0) * p.gt <= s.part_rows);
+                    CHECK(s.part_row >= 0 && s.part_row + span <= rows);
+                    for (int q = 0; q < span; ++q) CHECK(taken.insert(s.part_row + q).second);
                 }
                 units[Key(s.ctx, s.head0, s.tok0)].push_back({i, s});
             }
-            CHECK(n > 0 || x1 - x0 < p.min_per);
+            CHECK(n > 0 || x1 - x0 < per[line] || x1 - x0 < 2 * (kBlockKeys + kUnitCost));
         }
         size_t count = 0;
         for (int c = c_lo; c < p.B; ++c) {
@@ -143,7 +153,7 @@ int main(int argc, char** argv) {
                             CHECK(v[k].second.blk0 == at && (k == 0 || v[k].first == v[k - 1].first + 1));
                             at += v[k].second.n_blk;
                         }
-                        CHECK(at == unit_blocks(p, x, q));
+                        CHECK(at == (unit_keys(p, x, q) + kBlockKeys - 1) / kBlockKeys);
                         const int last = std::min((q + 1) * 2 * p.tpt, x.ntok) - 1;  // token of the context
                         CHECK(at * kBlockKeys >= (p.causal ? std::min(x.len, x.len - x.ntok + last + 1) : x.len));
                         if (p.prefix_mode) continue;
@@ -151,46 +161,41 @@ int main(int argc, char** argv) {
                             CHECK(v[0].second.part_row == -1);
                             continue;
                         }
-                        const Split& s = split[v[0].first];
+                        const bool few = v[0].second.mode == kFew;
+                        const Split& s = split[(few ? grid : 0) + v[0].first];
                         CHECK(s.last == v.back().first && s.tok0 == v[0].second.tok0 &&
                               s.head0 == v[0].second.head0 && s.mode == v[0].second.mode);
                         for (size_t k = 0; k < v.size(); ++k)
                             CHECK(v[k].second.part_row ==
-                                  (2 * (v[0].first + static_cast<int>(k)) + (k == 0 ? 1 : 0)) * 2 * kTileRows);
+                                  (few ? p.few_part_row : 0) +
+                                      (2 * (v[0].first + static_cast<int>(k)) + (k == 0 ? 1 : 0)) *
+                                          (few ? kFewTile : 2 * kTileRows));
                     }
         }
         CHECK(count == units.size());
         if (p.prefix_mode) {
-            const Ctx pre = load_ctx(p, -1);
-            for (int t = 0; t < 40; ++t) {
-                const int b = R(0, p.B - 1), h = R(0, p.hq - 1);
-                const Ctx own = load_ctx(p, b);
-                const int hk = h / group, ch = (h % group) / p.gt, hr = (h % group) % p.gt;
-                const PrefixParts q = prefix_parts(p, per, pre, own, b, hk * p.chunks + ch, hr);
-                const int tile = b / p.tpt;
-                if (pre.len > 0) {
-                    const auto& v = units[Key(-1, hk * group + ch * p.gt, (tile / 2) * 2 * p.tpt)];
-                    CHECK(static_cast<int>(v.size()) == q.n1 && q.r1 == (b % p.tpt) * p.gt + hr);
-                    for (int k = 0; k < q.n1; ++k) {
-                        CHECK(v[k].second.mode == kTwoTiles || tile % 2 == 0);
-                        CHECK(q.row1 + k * 2 * kTileRows == v[k].second.part_row + (tile % 2) * kTileRows);
-                    }
-                } else {
-                    CHECK(q.n1 == 0);
-                }
-                if (own.len > 0) {
-                    const auto& v = units[Key(b, hk * group + ch * p.gt, b)];
-                    CHECK(static_cast<int>(v.size()) == q.n2 && q.r2 == hr);
-                    for (int k = 0; k < q.n2; ++k) CHECK(q.row2 + k * p.gt == v[k].second.part_row);
-                } else {
-                    CHECK(q.n2 == 0);
+            for (const auto& u : units) {
+                const Seg& s0 = u.second[0].second;
+                const int hc = s0.hk * p.chunks + (s0.head0 - s0.hk * group) / p.gt;
+                const int pair = s0.ctx < 0 ? s0.tok0 / (2 * p.tpt) : 0;
+                const int n = s0.ctx < 0 ? hc * p.prefix_pairs + pair : heads * p.prefix_pairs + s0.ctx * heads + hc;
+                const Span sp = span[n];
+                CHECK(sp.first == u.second[0].first && sp.last == u.second.back().first);
+                // the second kernel's addresses
+                for (size_t k = 0; k < u.second.size(); ++k) {
+                    const int piece = sp.first + static_cast<int>(k);
+                    CHECK(u.second[k].second.part_row ==
+                          (s0.ctx < 0 ? (n + piece) * 2 * kTileRows
+                                      : p.own_part_row + (n - heads * p.prefix_pairs + piece) * p.gt));
                 }
             }
         } else {
-            for (int i = 0; i < grid; ++i) {
+            for (int i = 0; i < 2 * grid; ++i) {
                 if (split[i].last < 0) continue;
                 bool found = false;
-                for (const auto& u : units) found = found || (u.second.size() > 1 && u.second[0].first == i);
+                for (const auto& u : units)
+                    found = found || (u.second.size() > 1 && u.second[0].first == i % grid &&
+                                      (u.second[0].second.mode == kFew) == (i >= grid));
                 CHECK(found);
             }
         }
