@@ -1309,13 +1309,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// The second kernel: joins partial rows by their log2-sum-exp, in the order of
-// the line.  A block takes 32 rows (one per lane, so that loads of the
-// partials' layout are contiguous); its 8 warps share the columns, four at a
-// time, and the result is transposed through shared memory for its stores.
-// Bound by latency (dependent rounds of loads, instruction fetches), not bytes.
+// The second kernel: joins partial rows by their log2-sum-exp.  A block takes 32
+// rows (one per lane, so that loads of the partials' layout are contiguous) and
+// 32 columns; its 8 warps share the partials (warp w those at w, w + 8, ...),
+// and their sums are joined through shared memory in warp order, so a result
+// depends on the lengths alone.  Bound by latency: with the maxima, weights and
+// products of all partials in one warp after the other, 37 partials took 26 us,
+// this way one round of loads and one exchange.
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinCols = 32;
 
 // A lane's partials: n of them, tiles of `rows` rows `step` rows apart from
 // `base` on, row r of each.
@@ -1323,72 +1327,95 @@ struct Parts {
     int n, base, step, rows, r;
 };
 
-// Joins the partials of both lists for this block's 32 rows and writes them;
-// lane's row goes to out_row (-1: none).
+template <typename T>
+struct JoinSmem {
+    float4 acc[kJoinWarps][kJoinCols / 4][32];
+    float top[kJoinWarps][32];
+    float tot[kJoinWarps][32];
+    int row[32];
+    __align__(16) T tile[32][kJoinCols + 8];
+};
+
+// One partial into a lane's running maximum, sum and output.
+template <int D>
+__device__ __forceinline__ void join_part(const TcParams& p, int tile_row, int rows, int r, int col0, float& top,
+                                          float& tot, float4 (&acc)[kJoinCols / 4]) {
+    constexpr int Q = kJoinCols / 4;
+    const float lse = p.L_part[tile_row + r];
+    const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(tile_row) * D) +
+                        (col0 / 4) * rows + r;
+    float4 v[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) v[q] = src[q * rows];
+    const float m = fmaxf(top, lse);
+    const float m0 = m == -INFINITY ? 0.f : m;
+    const float w0 = sm100::ex2_approx(top - m0), w1 = sm100::ex2_approx(lse - m0);
+    top = m;
+    tot = tot * w0 + w1;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        acc[q].x = fmaf(w1, v[q].x, acc[q].x * w0);
+        acc[q].y = fmaf(w1, v[q].y, acc[q].y * w0);
+        acc[q].z = fmaf(w1, v[q].z, acc[q].z * w0);
+        acc[q].w = fmaf(w1, v[q].w, acc[q].w * w0);
+    }
+}
+
+// Joins the partials of both lists, a lane's row going to out_row (-1: none),
+// columns [col0, col0 + 32).
 template <typename T, int D>
-__device__ __forceinline__ void join_rows(const TcParams& p, const Parts& a, const Parts& b, int out_row) {
-    constexpr int Q = D / 4 / (kJoinThreads / 32);  // column quads per warp
-    constexpr int kFlight = 16 / Q;                 // partials in flight: 16 loads of 16 bytes
-    constexpr int kPitch = D + 8;  // 16-bit elements; rows 16 bytes apart in the banks
-    __shared__ __align__(16) T tile[32][kPitch];
-    __shared__ int out[32];
+__device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, const Parts& a, const Parts& b,
+                                          int out_row, int col0) {
+    constexpr int Q = kJoinCols / 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = a.n + b.n;
-    auto tile_row = [&](int k) -> int { return k < a.n ? a.base + k * a.step : b.base + (k - a.n) * b.step; };
-    float M = -INFINITY;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) M = fmaxf(M, p.L_part[tile_row(k) + (k < a.n ? a.r : b.r)]);
     float4 acc[Q];
-    float tot = 0.f;
+    float top = -INFINITY, tot = 0.f;
 #pragma unroll
     for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int k0 = 0; k0 < n && M != -INFINITY; k0 += kFlight) {
-        float4 v[kFlight][Q];
-        float w[kFlight];
+    for (int k = warp; k < n; k += kJoinWarps) {
+        const bool in_a = k < a.n;
+        const int at = in_a ? a.base + k * a.step : b.base + (k - a.n) * b.step;
+        const int r = in_a ? a.r : b.r, rows = in_a ? a.rows : b.rows;
+        join_part<D>(p, at, rows, r, col0, top, tot, acc);
+    }
+    __syncthreads();  // the last use of the shared memory is over
 #pragma unroll
-        for (int k = 0; k < kFlight; ++k) {
-            const int kk = min(k0 + k, n - 1);
-            const int at = tile_row(kk), r = kk < a.n ? a.r : b.r, rows = kk < a.n ? a.rows : b.rows;
-            w[k] = p.L_part[at + r];
-            const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(at) * D) + r +
-                                warp * Q * rows;
+    for (int q = 0; q < Q; ++q) sm.acc[warp][q][lane] = acc[q];
+    sm.top[warp][lane] = top;
+    sm.tot[warp][lane] = tot;
+    if (warp == 0) sm.row[lane] = out_row;
+    __syncthreads();
+    // warp q: columns 4 q .. 4 q + 3
+    float M = -INFINITY;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) v[k][q] = src[q * rows];
-        }
+    for (int u = 0; u < kJoinWarps; ++u) M = fmaxf(M, sm.top[u][lane]);
+    const float M0 = M == -INFINITY ? 0.f : M;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    tot = 0.f;
 #pragma unroll
-        for (int k = 0; k < kFlight; ++k) {
-            const float wk = k0 + k < n ? sm100::ex2_approx(w[k] - M) : 0.f;
-            tot += wk;
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                acc[q].x = fmaf(wk, v[k][q].x, acc[q].x);
-                acc[q].y = fmaf(wk, v[k][q].y, acc[q].y);
-                acc[q].z = fmaf(wk, v[k][q].z, acc[q].z);
-                acc[q].w = fmaf(wk, v[k][q].w, acc[q].w);
-            }
-        }
+    for (int u = 0; u < kJoinWarps; ++u) {
+        const float w = sm100::ex2_approx(sm.top[u][lane] - M0);
+        const float4 v = sm.acc[u][warp][lane];
+        tot = fmaf(w, sm.tot[u][lane], tot);
+        o.x = fmaf(w, v.x, o.x);
+        o.y = fmaf(w, v.y, o.y);
+        o.z = fmaf(w, v.z, o.z);
+        o.w = fmaf(w, v.w, o.w);
     }
     const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-        uint2 v;
-        v.x = DType<T>::pack2(acc[q].x * inv, acc[q].y * inv);
-        v.y = DType<T>::pack2(acc[q].z * inv, acc[q].w * inv);
-        *reinterpret_cast<uint2*>(&tile[lane][(warp * Q + q) * 4]) = v;
-    }
-    if (warp == 0) {
-        out[lane] = out_row;
-        if (out_row >= 0) p.L[out_row] = tot > 0.f ? (M + __log2f(tot)) * kLn2 : -INFINITY;
-    }
+    uint2 packed;
+    packed.x = DType<T>::pack2(o.x * inv, o.y * inv);
+    packed.y = DType<T>::pack2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(&sm.tile[lane][warp * 4]) = packed;
+    if (warp == 0 && col0 == 0 && out_row >= 0)
+        p.L[out_row] = tot > 0.f ? (M + __log2f(tot)) * kLn2 : -INFINITY;
     __syncthreads();
-#pragma unroll 1
-    for (int e = threadIdx.x; e < 32 * (D / 8); e += kJoinThreads) {
-        const int r = e / (D / 8), c = e % (D / 8);
-        if (out[r] >= 0)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(out[r]) * D + c * 8) =
-                *reinterpret_cast<const uint4*>(&tile[r][c * 8]);
-    }
+    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
+    if (r < 32 && sm.row[r] >= 0)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(sm.row[r]) * D + col0 + c) =
+            *reinterpret_cast<const uint4*>(&sm.tile[r][c]);
 }
 
 __device__ __forceinline__ bool partials_ready() {
@@ -1397,11 +1424,12 @@ __device__ __forceinline__ bool partials_ready() {
     return *reinterpret_cast<const volatile int*>(&g_paged_status.code) == 0;
 }
 
-// Block (head chunk, 32 rows of the batch's row tiles): the prefix's partials,
-// then the sequence's own.
+// Block (32 rows of the batch's row tiles, head chunk, 32 columns): the prefix's
+// partials, then the sequence's own.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_prefix_kernel(const __grid_constant__ TcParams p) {
+    __shared__ JoinSmem<T> sm;
     const PagedLine& ln = p.ln;
     const int hc = blockIdx.y;
     const int row = blockIdx.x * 32 + (threadIdx.x & 31);  // of the head chunk
@@ -1428,37 +1456,136 @@ __global__ void __launch_bounds__(kJoinThreads)
         const Span sp = ln.span[ln.heads * ln.prefix_pairs + u];
         own = Parts{sp.last - sp.first + 1, ln.own_part_row + (u + sp.first) * ln.gt, ln.gt, ln.gt, hr};
     }
-    join_rows<T, D>(p, pre, own, valid ? b * ln.hq + head : -1);
+    join_rows<T, D>(p, sm, pre, own, valid ? b * ln.hq + head : -1, blockIdx.z * kJoinCols);
 }
 
-// Block (i, y): rows [32 y, 32 y + 32) of the row tiles (y < 8), or the few
-// rows (y = 8), of the unit that piece i of the line had the first blocks of
-// and piece split.last the last.
+// The ragged units that several pieces share, 32 rows and 32 columns at a time.
+// Every block counts them (records split over its threads).  Units of few
+// partials, the usual kind, are joined by single warps, a lane per row, without
+// any exchange; the others by whole blocks as above.
+constexpr int kLightParts = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_split_kernel(const __grid_constant__ TcParams p) {
+    constexpr int kColGroups = D / kJoinCols;
+    __shared__ JoinSmem<T> sm;
+    __shared__ int ends[2][kJoinThreads + 1];  // [light, heavy]: items of the threads before
     const PagedLine& ln = p.ln;
     if (!partials_ready()) return;
-    const int i = static_cast<int>(blockIdx.x);
-    const bool few = blockIdx.y == 2 * kTileRows / 32;
-    const Split sp = ln.split[(few ? ln.pieces : 0) + i];
-    if (sp.last <= i) return;
-    const int row = (few ? 0 : blockIdx.y * 32) + (threadIdx.x & 31);
-    const int tile = row / kTileRows;
-    const int r = row % kTileRows;
-    if (tile == 1 && sp.mode != kTwoTiles) return;
-    const int tok_r = r / ln.gt;
-    const int hr = r - tok_r * ln.gt;
-    const int token = sp.tok0 + tile * ln.tpt + tok_r;
-    const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
-    if (__syncthreads_or(valid) == 0) return;
-    // piece i's last segment, then the first ones of the pieces behind it
-    const int rows = few ? kFewTile : kTileRows;      // of a tile
-    const int slot = few ? kFewTile : 2 * kTileRows;  // of a segment
-    const int base = (few ? ln.few_part_row : tile * kTileRows) + 2 * i * slot;
-    const Parts head = {valid ? 1 : 0, base + slot, 0, rows, r};
-    const Parts rest = {valid ? sp.last - i : 0, base + 2 * slot, 2 * slot, rows, r};
-    join_rows<T, D>(p, head, rest, valid ? token * ln.hq + sp.head0 + hr : -1);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n_rec = 2 * ln.pieces;
+    const int run = (n_rec + kJoinThreads - 1) / kJoinThreads;
+    auto piece_of = [&](int i) -> int { return i < ln.pieces ? i : i - ln.pieces; };
+    // items of record i: groups of 32 rows times groups of columns
+    auto items = [&](int i, int kind) -> int {
+        if (i >= n_rec) return 0;
+        const Split sp = ln.split[i];
+        const int n = sp.last - piece_of(i) + 1;
+        if (n <= 1 || (n > kLightParts) != (kind == 1)) return 0;
+        const int tokens = min(sp.tok_end - sp.tok0, sp.mode == kTwoTiles ? 2 * ln.tpt : ln.tpt);
+        const int rows = tokens > ln.tpt ? kTileRows + (tokens - ln.tpt) * ln.gt : tokens * ln.gt;
+        return (rows + 31) / 32 * kColGroups;
+    };
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+        int mine = 0;
+#pragma unroll 1
+        for (int k = 0; k < run; ++k) mine += items(threadIdx.x * run + k, kind);
+        ends[kind][threadIdx.x + 1] = mine;
+    }
+    __syncthreads();
+    if (warp < 2) {  // inclusive sums, 8 threads' counts per lane
+        int v[kJoinThreads / 32], sum = 0;
+#pragma unroll
+        for (int k = 0; k < kJoinThreads / 32; ++k) {
+            sum += ends[warp][1 + lane * (kJoinThreads / 32) + k];
+            v[k] = sum;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += u;
+        }
+#pragma unroll
+        for (int k = 0; k < kJoinThreads / 32; ++k)
+            ends[warp][1 + lane * (kJoinThreads / 32) + k] = v[k] + incl - sum;
+        if (lane == 0) ends[warp][0] = 0;
+    }
+    __syncthreads();
+    struct Item {
+        Parts head, rest;
+        int out_row, col0;
+    };
+    // item `at` of a kind, for this lane's row; the whole warp takes part
+    auto find = [&](int at, int kind) -> Item {
+        int owner = 0;
+#pragma unroll
+        for (int k = 0; k < kJoinThreads / 32; ++k) {
+            const int th = k * 32 + lane;
+            const unsigned hit = __ballot_sync(0xffffffffu, ends[kind][th] <= at && at < ends[kind][th + 1]);
+            if (hit != 0) owner = k * 32 + __ffs(hit) - 1;
+        }
+        int left = at - ends[kind][owner], rec = owner * run;
+        int n = items(rec, kind);
+#pragma unroll 1
+        while (left >= n) {
+            left -= n;
+            n = items(++rec, kind);
+        }
+        const Split sp = ln.split[rec];
+        const bool few = rec >= ln.pieces;
+        const int i = piece_of(rec);
+        const int row = left / kColGroups * 32 + lane;
+        const int tile = row / kTileRows;
+        const int r = row % kTileRows;
+        const int tok_r = r / ln.gt;
+        const int hr = r - tok_r * ln.gt;
+        const int token = sp.tok0 + tile * ln.tpt + tok_r;
+        const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
+        // piece i's last segment, then the first ones of the pieces behind it
+        const int rows = few ? kFewTile : kTileRows;      // of a tile
+        const int slot = few ? kFewTile : 2 * kTileRows;  // of a segment
+        const int base = (few ? ln.few_part_row : tile * kTileRows) + 2 * i * slot;
+        return Item{Parts{valid ? 1 : 0, base + slot, 0, rows, r},
+                    Parts{valid ? sp.last - i : 0, base + 2 * slot, 2 * slot, rows, r},
+                    valid ? token * ln.hq + sp.head0 + hr : -1, left % kColGroups * kJoinCols};
+    };
+    const int light = ends[0][kJoinThreads], heavy = ends[1][kJoinThreads];
+#pragma unroll 1
+    for (int at = blockIdx.x; at < heavy; at += gridDim.x) {
+        const Item it = find(at, 1);
+        join_rows<T, D>(p, sm, it.head, it.rest, it.out_row, it.col0);
+    }
+#pragma unroll 1
+    for (int at = blockIdx.x * kJoinWarps + warp; at < light; at += gridDim.x * kJoinWarps) {
+        const Item it = find(at, 0);
+        if (it.out_row < 0) continue;
+        constexpr int Q = kJoinCols / 4;
+        float4 acc[Q];
+        float top = -INFINITY, tot = 0.f;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int n = it.rest.n + 1;
+#pragma unroll 1
+        for (int k = 0; k < n; ++k) {
+            const int tile_row = k == 0 ? it.head.base : it.rest.base + (k - 1) * it.rest.step;
+            join_part<D>(p, tile_row, it.head.rows, it.head.r, it.col0, top, tot, acc);
+        }
+        const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(it.out_row) * D + it.col0);
+#pragma unroll
+        for (int q = 0; q < Q; q += 2) {
+            uint4 v;
+            v.x = DType<T>::pack2(acc[q].x * inv, acc[q].y * inv);
+            v.y = DType<T>::pack2(acc[q].z * inv, acc[q].w * inv);
+            v.z = DType<T>::pack2(acc[q + 1].x * inv, acc[q + 1].y * inv);
+            v.w = DType<T>::pack2(acc[q + 1].z * inv, acc[q + 1].w * inv);
+            dst[q / 2] = v;
+        }
+        if (it.col0 == 0) p.L[it.out_row] = tot > 0.f ? (top + __log2f(tot)) * kLn2 : -INFINITY;
+    }
 }
 
 // Launches `kern` so that its blocks may be scheduled while the kernel before
@@ -1507,7 +1634,7 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     p.few_tok = std::max(1, kFewRows / ln.gt);
     const int grid = persistent_grid(0x7fffffffLL, 1);
     long long rows, records;
-    if (!set_parts(ln, grid, rows, records)) return FlashAttentionError::INVALID_DIMENSION;
+    if (!set_parts(ln, grid, rows, records) || ln.heads > 65535) return FlashAttentionError::INVALID_DIMENSION;
 
     const CUtensorMapDataType dt = DType<T>::kTmaType;
     const CUtensorMapSwizzle swz = G::kSwz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -1558,10 +1685,10 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
             const int tiles = (ln.B + ln.tpt - 1) / ln.tpt;
             const int last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
             const int groups = (tiles - 1) * (kTileRows / 32) + (last + 31) / 32;
-            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads), stream, p);
+            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kJoinCols), stream, p);
         } else {
-            err = launch_behind(paged_join_split_kernel<T, D>,
-                                dim3(grid, 2 * kTileRows / 32 + (G::kHasFew ? 1 : 0)), stream, p);
+            // as many blocks as are resident at once (two per SM)
+            err = launch_behind(paged_join_split_kernel<T, D>, dim3(2 * grid), stream, p);
         }
         if (err != cudaSuccess) cudaGetLastError();
     }
