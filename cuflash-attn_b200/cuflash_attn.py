@@ -178,52 +178,55 @@ def rope_table(max_position: int, rotary_dim: int, base: float = 10000.0, device
     return torch.cat([angle.cos(), angle.sin()], dim=1).to(device, torch.float32)
 
 
-def _token_stride(t) -> int:
-    """Elements between tokens of t [tokens, heads, D] whose heads are packed
-    (0 where there is only one)."""
-    tokens, heads, D = t.shape
-    between, head, element = t.stride()
-    if element != 1 or (heads > 1 and head != D):
-        raise ValueError("a token's heads must be contiguous")
-    if tokens <= 1:
-        return 0
-    if between < heads * D:
-        raise ValueError("tokens must not overlap")
-    return between
-
-
-# The checks of the paged-cache entries, which run once per token of a serving
-# loop: device numbers, dtypes and sizes are compared with as few calls into
-# torch as there are tensors, and what is wrong is only worked out for the error.
-def _check_packed(dtype, **tensors) -> None:
-    """Contiguous tensors of one type."""
-    for name, t in tensors.items():
-        if t.dtype is not dtype:
-            raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {dtype}, not {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-
-
-def _check_device(device: int, *tensors) -> None:
-    """All on CUDA device `device` (-1: the first one is on none)."""
+# Checks of the paged-cache entries, which run once per token of a serving loop:
+# a tensor that passes costs three calls into torch (type, device, packing), and
+# what is wrong is only worked out for the error.
+def _packed_on(device: int, dtype, tensors) -> bool:
     for t in tensors:
-        if t.get_device() != device or device < 0:
-            raise ValueError(f"every tensor must be on one CUDA device, not {t.device}")
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+            return False
+    return device >= 0
+
+
+def _require(device: int, *groups) -> None:
+    """Raises what is wrong with contiguous tensors of one type and device:
+    groups of (dtype, {name: tensor}); types first, then layouts, then devices."""
+    for dtype, tensors in groups:
+        for name, t in tensors.items():
+            if t.dtype is not dtype:
+                raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {dtype}, not {t.dtype}")
+    for _, tensors in groups:
+        for name, t in tensors.items():
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+    for _, tensors in groups:
+        for name, t in tensors.items():
+            if t.get_device() != device or device < 0:
+                raise ValueError(f"{name} must be on one CUDA device with the others, not {t.device}")
 
 
 def _mismatch(name, t, shape):
     return CuFlashError(DIMENSION_MISMATCH, f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
 
 
-def _run_on(device: int, stream, call):
-    """call(raw stream) with `device` current; by default on its current stream."""
-    import torch
-
-    raw = (torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
-    if torch._C._cuda_getDevice() == device:
-        return call(raw)
-    with torch.cuda.device(device):
-        return call(raw)
+def _token_stride(t, dtype, device: int, shape, name: str) -> int:
+    """Elements between tokens of t [tokens, heads, D] whose heads are packed
+    (0 where there is only one); t like `shape`, on `device`."""
+    if t.shape != shape:
+        raise _mismatch(name, t, shape)
+    if t.dtype is not dtype:
+        raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {dtype}, not {t.dtype}")
+    tokens, heads, D = shape
+    between, head, element = t.stride()
+    if element != 1 or (heads > 1 and head != D):
+        raise ValueError("a token's heads must be contiguous")
+    if t.get_device() != device or device < 0:
+        raise ValueError(f"{name} must be on one CUDA device with the others, not {t.device}")
+    if tokens <= 1:
+        return 0
+    if between < heads * D:
+        raise ValueError("tokens must not overlap")
+    return between
 
 
 class CuFlashAttn:
@@ -232,6 +235,29 @@ class CuFlashAttn:
 
     def __init__(self, lib_path: Optional[str] = None, reference_abi_only: bool = False):
         self.lib = load_library(lib_path, reference_abi_only)
+        self._paged_fn = {}  # (entry, dtype) -> C function
+
+    def _paged(self, entry: str, t):
+        key = (entry, t.dtype)
+        fn = self._paged_fn.get(key)
+        if fn is None:
+            fn = self._paged_fn[key] = getattr(self.lib, f"{entry}_{_suffix(t)}")
+        return fn
+
+    def _call_on(self, device: int, stream, fn, *args) -> None:
+        """fn(*args, stream) with `device` current; by default on its current
+        stream."""
+        import torch
+
+        raw = (torch._C._cuda_getCurrentRawStream(device) if stream is None
+               else stream.cuda_stream)
+        if torch._C._cuda_getDevice() == device:
+            code = fn(*args, raw)
+        else:
+            with torch.cuda.device(device):
+                code = fn(*args, raw)
+        if code:
+            self.check_error(code)
 
     def error_string(self, code: int) -> str:
         return self.lib.cuflash_error_string(int(code)).decode("utf-8")
@@ -369,54 +395,47 @@ class CuFlashAttn:
             raise _mismatch("V_cache", V_cache, K_cache.shape)
         if seq_lens.shape != (B,):
             raise _mismatch("seq_lens", seq_lens, (B,))
-        if V.dtype is not dtype:
-            raise CuFlashError(UNSUPPORTED_DTYPE, f"V must be {dtype}, not {V.dtype}")
-        _check_packed(dtype, K_cache=K_cache, V_cache=V_cache)
-        _check_packed(torch.int32, block_table=block_table, seq_lens=seq_lens)
-        k_stride, v_stride, q_stride = _token_stride(K), _token_stride(V), 0
-        Hq = q_ptr = out_ptr = cu_ptr = pos_ptr = rope_ptr = max_position = rotary = 0
+        ints = (block_table, seq_lens)
+        cu_ptr = pos_ptr = 0
         if cu_seqlens is not None:
             if cu_seqlens.shape != (B + 1,):
                 raise _mismatch("cu_seqlens", cu_seqlens, (B + 1,))
-            _check_packed(torch.int32, cu_seqlens=cu_seqlens)
-            _check_device(device, cu_seqlens)
+            ints += (cu_seqlens,)
             cu_ptr = cu_seqlens.data_ptr()
         if positions is not None:
             if positions.shape != (tokens,):
                 raise _mismatch("positions", positions, (tokens,))
-            _check_packed(torch.int32, positions=positions)
-            _check_device(device, positions)
+            ints += (positions,)
             pos_ptr = positions.data_ptr()
+        if not (_packed_on(device, torch.int32, ints)
+                and _packed_on(device, dtype, (K_cache, V_cache))):
+            _require(device, (dtype, {"K_cache": K_cache, "V_cache": V_cache}),
+                     (torch.int32, {f"index tensor {i}": t for i, t in enumerate(ints)}))
+        k_stride = _token_stride(K, dtype, device, shape, "K")
+        v_stride = _token_stride(V, dtype, device, shape, "V")
+        Hq = q_stride = q_ptr = out_ptr = rope_ptr = max_position = rotary = 0
         if Q is not None:
             Hq = Q.shape[1]
-            if Q.shape != (tokens, Hq, D):
-                raise _mismatch("Q", Q, (tokens, Hq, D))
-            if Q.dtype is not dtype:
-                raise CuFlashError(UNSUPPORTED_DTYPE, f"Q must be {dtype}, not {Q.dtype}")
-            q_stride = _token_stride(Q)
+            q_stride = _token_stride(Q, dtype, device, (tokens, Hq, D), "Q")
             if Q_out is None:
                 Q_out = torch.empty((tokens, Hq, D), device=Q.device, dtype=dtype)
             elif Q_out.shape != Q.shape:
                 raise _mismatch("Q_out", Q_out, Q.shape)
-            _check_packed(dtype, Q_out=Q_out)
-            _check_device(device, Q, Q_out)
+            elif not _packed_on(device, dtype, (Q_out,)):
+                _require(device, (dtype, {"Q_out": Q_out}))
             q_ptr, out_ptr = Q.data_ptr(), Q_out.data_ptr()
         elif Q_out is not None:
             raise ValueError("Q_out without Q")
         if rope_table is not None:
-            _check_packed(torch.float32, rope_table=rope_table)
-            _check_device(device, rope_table)
+            if not _packed_on(device, torch.float32, (rope_table,)):
+                _require(device, (torch.float32, {"rope_table": rope_table}))
             max_position, rotary = rope_table.shape
             rope_ptr = rope_table.data_ptr()
-        _check_device(device, K, V, K_cache, V_cache, block_table, seq_lens)
-        fn = getattr(self.lib, "cuflash_kv_append_paged_" + _suffix(K))
-        code = _run_on(device, stream, lambda raw: fn(
-            q_ptr, K.data_ptr(), V.data_ptr(), out_ptr, K_cache.data_ptr(), V_cache.data_ptr(),
-            rope_ptr, pos_ptr, block_table.data_ptr(), seq_lens.data_ptr(), cu_ptr, tokens, B, Hq,
-            Hkv, D, page_size, max_pages, num_pages, q_stride, k_stride, v_stride, rotary,
-            max_position, interleaved, raw))
-        if code:
-            self.check_error(code)
+        self._call_on(device, stream, self._paged("cuflash_kv_append_paged", K), q_ptr,
+                      K.data_ptr(), V.data_ptr(), out_ptr, K_cache.data_ptr(),
+                      V_cache.data_ptr(), rope_ptr, pos_ptr, block_table.data_ptr(),
+                      seq_lens.data_ptr(), cu_ptr, tokens, B, Hq, Hkv, D, page_size, max_pages,
+                      num_pages, q_stride, k_stride, v_stride, rotary, max_position, interleaved)
         return Q_out
 
     def forward_paged(self, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens,
@@ -439,19 +458,17 @@ class CuFlashAttn:
             raise _mismatch("seq_lens", seq_lens, (B,))
         if cu_seqlens.shape != (B + 1,):
             raise _mismatch("cu_seqlens", cu_seqlens, (B + 1,))
-        _check_packed(dtype, Q=Q, K_cache=K_cache, V_cache=V_cache)
-        _check_packed(torch.int32, block_table=block_table, seq_lens=seq_lens,
-                      cu_seqlens=cu_seqlens)
-        _check_device(device, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens)
-        O, L = self._outputs(Q, shape, (tokens, Hq), O, L)
-        fn = getattr(self.lib, "cuflash_attention_forward_paged_" + _suffix(Q))
-        code = _run_on(device, stream, lambda raw: fn(
-            Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), block_table.data_ptr(),
-            seq_lens.data_ptr(), cu_seqlens.data_ptr(), O.data_ptr(), L.data_ptr(), tokens, B, Hq,
-            Hkv, D, page_size, max_pages, num_pages,
-            D ** -0.5 if scale is None else scale, causal, raw))
-        if code:
-            self.check_error(code)
+        if not (_packed_on(device, dtype, (Q, K_cache, V_cache))
+                and _packed_on(device, torch.int32, (block_table, seq_lens, cu_seqlens))):
+            _require(device, (dtype, {"Q": Q, "K_cache": K_cache, "V_cache": V_cache}),
+                     (torch.int32, {"block_table": block_table, "seq_lens": seq_lens,
+                                    "cu_seqlens": cu_seqlens}))
+        O, L = self._outputs(Q, device, shape, (tokens, Hq), O, L)
+        self._call_on(device, stream, self._paged("cuflash_attention_forward_paged", Q),
+                      Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
+                      block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
+                      O.data_ptr(), L.data_ptr(), tokens, B, Hq, Hkv, D, page_size, max_pages,
+                      num_pages, D ** -0.5 if scale is None else scale, causal)
         return O, L
 
     def decode_shared_prefix(self, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
@@ -480,42 +497,37 @@ class CuFlashAttn:
             raise _mismatch("seq_lens", seq_lens, (B,))
         if prefix_len.shape != (1,):
             raise _mismatch("prefix_len", prefix_len, (1,))
-        _check_packed(dtype, q=q, K_cache=K_cache, V_cache=V_cache)
-        _check_packed(torch.int32, prefix_table=prefix_table, prefix_len=prefix_len,
-                      block_table=block_table, seq_lens=seq_lens)
-        _check_device(device, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
-                      seq_lens)
-        O, L = self._outputs(q, shape, (B, Hq), O, L)
-        fn = getattr(self.lib, "cuflash_attention_decode_shared_prefix_" + _suffix(q))
-        code = _run_on(device, stream, lambda raw: fn(
-            q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_table.data_ptr(),
-            prefix_len.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), O.data_ptr(),
-            L.data_ptr(), B, Hq, Hkv, D, page_size, max_prefix, max_pages, num_pages,
-            D ** -0.5 if scale is None else scale, raw))
-        if code:
-            self.check_error(code)
+        if not (_packed_on(device, dtype, (q, K_cache, V_cache))
+                and _packed_on(device, torch.int32,
+                               (prefix_table, prefix_len, block_table, seq_lens))):
+            _require(device, (dtype, {"q": q, "K_cache": K_cache, "V_cache": V_cache}),
+                     (torch.int32, {"prefix_table": prefix_table, "prefix_len": prefix_len,
+                                    "block_table": block_table, "seq_lens": seq_lens}))
+        O, L = self._outputs(q, device, shape, (B, Hq), O, L)
+        self._call_on(device, stream, self._paged("cuflash_attention_decode_shared_prefix", q),
+                      q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
+                      prefix_table.data_ptr(), prefix_len.data_ptr(), block_table.data_ptr(),
+                      seq_lens.data_ptr(), O.data_ptr(), L.data_ptr(), B, Hq, Hkv, D, page_size,
+                      max_prefix, max_pages, num_pages, D ** -0.5 if scale is None else scale)
         return O, L
 
     @staticmethod
-    def _outputs(q, o_shape, l_shape, O, L):
+    def _outputs(q, device, o_shape, l_shape, O, L):
         """O like q and L fp32, checked where the caller gave them."""
         import torch
 
-        device = q.get_device()
         if O is None:
             O = torch.empty_like(q)
-        else:
-            if O.shape != o_shape:
-                raise _mismatch("O", O, o_shape)
-            _check_packed(q.dtype, O=O)
-            _check_device(device, O)
+        elif O.shape != o_shape:
+            raise _mismatch("O", O, o_shape)
+        elif not _packed_on(device, q.dtype, (O,)):
+            _require(device, (q.dtype, {"O": O}))
         if L is None:
-            L = torch.empty(l_shape, device=q.device, dtype=torch.float32)
-        else:
-            if L.shape != l_shape:
-                raise _mismatch("L", L, l_shape)
-            _check_packed(torch.float32, L=L)
-            _check_device(device, L)
+            L = q.new_empty(l_shape, dtype=torch.float32)
+        elif L.shape != l_shape:
+            raise _mismatch("L", L, l_shape)
+        elif not _packed_on(device, torch.float32, (L,)):
+            _require(device, (torch.float32, {"L": L}))
         return O, L
 
     def forward_gqa(self, Q, K, V, causal: bool = False, scale: Optional[float] = None, O=None,
