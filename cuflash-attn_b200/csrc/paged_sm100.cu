@@ -198,8 +198,8 @@ FlashAttentionError paged_row(const PagedParams<T>& p, cudaStream_t stream) {
 //               are live (8 cycles each on the MUFU pipe of its quarter);
 //               here 128 threads on four quarters share them, and the result's
 //               rows lie across the lanes, so they are stored coalesced.
-//   warp 0      TMA producer: query tiles, K/V blocks through a ring of
-//               slots, one box per page and 64 columns, one lane each
+//   warps 0, 3  TMA producers (query tiles and keys; values): blocks through
+//               a ring of slots, one box per page and 64 columns, a lane each
 //   warp 1      tcgen05.mma issuer: S(n+2) behind O(n)
 //   warp 2      walks the line and hands out segments
 //   warps 4-11  softmax and epilogue
@@ -377,7 +377,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const PagedLine& ln = p.ln;
     // the joining kernel's blocks may wait on the SMs this one leaves
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (cta_skip(&g_paged_status)) return;
+    // what the plan reads is on its way while the barriers are set up
+    const int c_lo = ln.prefix_mode ? -1 : 0;
+    const int run = (ln.B - c_lo + kTcThreads - 1) / kTcThreads;  // contexts per thread
+    const int c_first = c_lo + static_cast<int>(threadIdx.x) * run;
+    if (c_first < ln.B) {
+        const int* at = c_first < 0 ? ln.prefix_len : ln.seq_lens + c_first;
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+        if (!ln.prefix_mode) asm volatile("prefetch.global.L1 [%0];" ::"l"(ln.cu_seqlens + c_first));
+    }
+    int failed = 0;  // an earlier launch's failure
+    if (threadIdx.x == 0) failed = *reinterpret_cast<const volatile int*>(&g_paged_status.code);
 
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_init(bar_y, 128);
         for (int s = 0; s < kSegRing; ++s) {
             mbar_init(seg_full + s, 1);
-            mbar_init(seg_free + s, 10);  // producer, MMA, 8 softmax warps
+            mbar_init(seg_free + s, 11);  // producers, MMA, 8 softmax warps
         }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
@@ -434,17 +444,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         prefetch_tmap(&tmQf);
         fence_mbar_init();
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
 
     // ---- the lines: contexts' lengths summed over the block, then the context
     // each of this CTA's pieces starts in
-    const int c_lo = ln.prefix_mode ? -1 : 0;
     const int n_cta = static_cast<int>(gridDim.x);
-    const int run = (ln.B - c_lo + kTcThreads - 1) / kTcThreads;  // contexts per thread
-    const int c_first = c_lo + static_cast<int>(threadIdx.x) * run;
     long long mine[2] = {0, 0};  // pass 0: lengths; pass 1: position behind the contexts so far
     Ctx ctx = {};
 #pragma unroll 1
@@ -477,7 +480,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 31) scan[l * 12 + warp] = incl;
             mine[l] = incl - mine[l];
         }
-        __syncthreads();
+        if (__syncthreads_or(failed)) return;
+        if (warp == 1) {
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        }
         long long sum[2] = {0, 0};
 #pragma unroll 1
         for (int w = 0; w < kTcThreads / 32; ++w) {
@@ -535,22 +542,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // 128 * 72 + 256 * 216 = 64512.
     if (warp < 4) {
         setmaxnreg_dec<72>();
-        if (warp == 0) {
-            // ------------------------------------------------ TMA producer
+        if (warp == 0 || warp == 3) {
+            // ------------------------------------------------ TMA producers
+            // Warp 0 loads query tiles and keys, warp 3 values: with 16-row pages
+            // one warp needs 0.7 us to issue the 16 boxes of a tile.
+            const int v = warp == 0 ? 0 : 1;
+            const CUtensorMap* map = v == 0 ? &tmK : &tmV;
             uint32_t q_cnt[2] = {0u, 0u};
-            uint32_t kv = 0;  // ring fills
-            int qs = 0;       // query slot of the next segment of one tile
+            // this warp's fills are every other one of the ring: fill `fills` + v in
+            // slot slot_kv; `phase`: parity of the slot's release before it
+            int slot_kv = v, fills = 0;
+            uint32_t phase = 1;
+            int qs = 0;  // query slot of the next segment of one tile
             const int box_rows = min(1 << ln.page_shift, kBlockKeys);
-            const int boxes = kBlockKeys / box_rows;  // per block and column block, <= 16
+            const int box_shift = min(ln.page_shift, 7);
+            const int chunk_shift = box_shift - 2;      // log2 of key blocks per 32 boxes
             const int my_box = lane & 15;
             const int my_cb = lane >> 4;
+            uint8_t* const my_dst = sptr + G::kOffRing + my_cb * G::kCbBytes + my_box * box_rows * G::kSwz;
             // Table entries come 32 boxes at a time, one per lane, a chunk ahead
             // (and the first of the next segment with this one's last block), so
             // that no copy waits for its page's index.
             auto load_entry = [&](const Seg& sg, int chunk) -> int {
                 const int* table = sg.ctx < 0 ? p.prefix_table
                                               : p.block_table + static_cast<long long>(sg.ctx) * ln.max_pages;
-                const long long row = (static_cast<long long>(chunk) * 32 + lane) * box_rows;
+                const long long row = (static_cast<long long>(chunk) * 32 + lane) << box_shift;
                 return row < sg.len ? table[row >> ln.page_shift] : 0;
             };
             int entry_next_seg = 0;
@@ -565,20 +581,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
                 if (sg.n_blk == 0) break;
                 since = tick();
-                int chunk = sg.blk0 * boxes / 32;
-                int entry = have_next ? entry_next_seg : load_entry(sg, chunk);
+                int chunk = sg.blk0 >> chunk_shift;
+                int entry = entry_next_seg;
+                if (!have_next) entry = load_entry(sg, chunk);
                 int entry_after = load_entry(sg, chunk + 1);
                 have_next = false;
                 // query tiles
-                if (lane == 0) {
+                if (lane == 0 && v == 0) {
                     const bool few = sg.mode == kFew;
                     const uint32_t bytes =
                         static_cast<uint32_t>(ln.gt * (few ? p.few_tok : ln.tpt)) * G::kRowBytes;
 #pragma unroll 1
                     for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
                         const int slot = sg.mode == kTwoTiles ? u : qs;
-                        if (q_cnt[slot] > 0)
-                            ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20);
+                        if (q_cnt[slot] > 0) ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20);
                         if (!ok) break;
                         mbar_arrive_expect_tx(bar_q + slot, bytes);
                         for (int cb = 0; cb < G::kNumCb; ++cb)
@@ -592,7 +608,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
                 for (int j = 0; ok && j < sg.n_blk; ++j) {
                     const int blk = sg.blk0 + j;
-                    if (blk * boxes / 32 != chunk) {
+                    if (blk >> chunk_shift != chunk) {
                         ++chunk;
                         entry = entry_after;
                         entry_after = load_entry(sg, chunk + 1);
@@ -600,48 +616,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (j + 1 == sg.n_blk &&
                         __all_sync(0xffffffffu, mbar_test(seg_full + (k + 1) % kSegRing,
                                                           ((k + 1) / kSegRing) & 1))) {
-                        const Seg nx = segs[(k + 1) % kSegRing];
+                        const Seg& nx = segs[(k + 1) % kSegRing];
                         if (nx.n_blk > 0) {
-                            entry_next_seg = load_entry(nx, nx.blk0 * boxes / 32);
+                            entry_next_seg = load_entry(nx, nx.blk0 >> chunk_shift);
                             have_next = true;
                         }
                     }
                     const int r0 = blk * kBlockKeys;
                     const int live = min(max(sg.len - r0, 0), kBlockKeys);
-                    const int nbox = (live + box_rows - 1) / box_rows;
+                    const int nbox = (live + box_rows - 1) >> box_shift;
+                    const int row = r0 + (my_box << box_shift);
                     // a page index outside the pool reads a wrong page instead of faulting
-                    const int page = min(max(__shfl_sync(0xffffffffu, entry, (blk * boxes + my_box) & 31), 0),
+                    const int page = min(max(__shfl_sync(0xffffffffu, entry, (row >> box_shift) & 31), 0),
                                          p.num_pages - 1);
-                    const int row0 = (page << ln.page_shift) +
-                                     ((r0 + my_box * box_rows) & ((1 << ln.page_shift) - 1));
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const int s = kv % R;
-                        if (lane == 0) {
-                            if (kv >= static_cast<uint32_t>(R))
-                                ok = poll_idle(empty + s, (kv / R - 1) & 1, 20);
-                            if (ok)
-                                mbar_arrive_expect_tx(full + s, static_cast<uint32_t>(nbox * box_rows) *
-                                                                    G::kRowBytes);
-                        }
-                        ok = __shfl_sync(0xffffffffu, ok, 0);
-                        if (!ok) break;
-                        if (my_box < nbox && my_cb < G::kNumCb)
-                            tma_load_3d(sptr + G::kOffRing + s * G::kTileBytes + my_cb * G::kCbBytes +
-                                            my_box * box_rows * G::kSwz,
-                                        v == 0 ? &tmK : &tmV, full + s, my_cb * G::kCbElems, sg.hk,
-                                        row0);
-                        ++kv;
+                    const int row0 = (page << ln.page_shift) + (row & ((1 << ln.page_shift) - 1));
+                    if (lane == 0) {
+                        // the first lap's waits pass: no fill has used the slot
+                        if (fills + v >= R) ok = poll_idle(empty + slot_kv, phase, 20);
+                        if (ok)
+                            mbar_arrive_expect_tx(full + slot_kv,
+                                                  static_cast<uint32_t>(nbox << box_shift) * G::kRowBytes);
                     }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+                    if (my_box < nbox && my_cb < G::kNumCb)
+                        tma_load_3d(my_dst + slot_kv * G::kTileBytes, map, full + slot_kv, my_cb * G::kCbElems,
+                                    sg.hk, row0);
+                    slot_kv += 2;
+                    if (slot_kv >= R) {
+                        slot_kv -= R;
+                        phase ^= 1;
+                    }
+                    fills += 2;
                 }
                 if (!ok) break;
             }
-            // every issued load lands before the CTA can exit
+            // Every issued load lands before the CTA can exit: those of this warp's
+            // fills that are the newest of their slots (older ones were consumed).
             if (lane == 0) {
                 volatile int never = 0;
                 for (int t = 0; t < 2; ++t)
                     if (q_cnt[t] > 0) mbar_wait(bar_q + t, (q_cnt[t] - 1) & 1, &never, &g_paged_status);
-                for (uint32_t g = kv > R ? kv - R : 0; g < kv; ++g)
+                const int old = max(fills - R - v, 0);
+                for (int g = old + (old & 1) + v; g < fills; g += 2)
                     mbar_wait(full + g % R, (g / R) & 1, &never, &g_paged_status);
             }
             __syncwarp();
@@ -779,20 +796,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     par ^= 1u << t;
                     return true;
                 };
-                // Stream t's turn: its O, then its next S behind it (in order, so
-                // that S may overwrite P).  With few rows the loads set the pace: the
-                // other stream's O does not wait behind an S whose keys have not
-                // landed; and the segment's products end before the next segment
-                // begins, which may need the query slot that holds P^T.
+                // The streams' turns: O of one, then its next S behind it (in order,
+                // so that S may overwrite P).
 #pragma unroll 1
                 for (int t = 0;; t ^= 1) {
                     const uint32_t mine = (due >> (16 * t)) & 0xffffu;
                     if (mine != 0 && !issue_o(t, mine)) break;
+                    // The other stream's O does not wait behind an S whose keys have
+                    // not landed; and a segment of few rows ends with all its
+                    // products, as the next one may need the query slot that holds P^T.
                     uint32_t other = (due >> (16 * (t ^ 1))) & 0xffffu;
-                    if (G::kHasFew && mode == kFew && other != 0 &&
-                        (i == steps || !__all_sync(0xffffffffu, mbar_test(full + ks, kph)))) {
-                        if (!issue_o(t ^ 1, other)) break;
-                        other = 0;
+                    if (other != 0) {
+                        bool now = G::kHasFew && mode == kFew && i == steps;
+#pragma unroll 1
+                        while (!now && i != steps && !__any_sync(0xffffffffu, mbar_test(full + ks, kph))) {
+                            now = __any_sync(0xffffffffu, mbar_test(bar_p + (t ^ 1), (par >> (t ^ 1)) & 1));
+                            if (__any_sync(0xffffffffu, *abort_flag != 0 || tick() - since > kWaitTicks)) break;
+                        }
+                        if (now) {
+                            if (!issue_o(t ^ 1, other)) break;
+                            other = 0;
+                        }
                     }
                     const uint32_t next = end ? 0 : issue_s(t);
                     due = (next << (16 * t)) | (other << (16 * (t ^ 1)));
