@@ -313,8 +313,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Converged-warp forms of the tcgen05 instructions: issued by the lane whose
-// `leader` is set (elect_lane, once per role).
+// For a converged warp of which one lane issues (`leader`, elected once per
+// role): the products stand under one branch, their operands are computed by
+// all lanes before it and stay in uniform registers.
 __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t p;
     asm volatile(
@@ -327,26 +328,6 @@ __device__ __forceinline__ uint32_t elect_lane() {
 template <typename V>
 __device__ __forceinline__ V uniform(V v) {
     return __shfl_sync(0xffffffffu, v, 0);
-}
-__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 e, %5, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
-        : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 e, %5, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
-        : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
     asm volatile(
@@ -733,15 +714,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const uint64_t b0 = pg_kdesc<D>(sb + G::kOffRing + ks * G::kTileBytes);
                     uint32_t flags = kDue | (i >= 2 ? kAcc : 0) | (i + 2 >= steps ? kLast : 0);
                     if (G::kHasFew && mode == kFew) {
+                        if (leader)
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            mma_ss(leader, tm + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
+                            mma_f16_ss(tm + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
                                        kk > 0 ? 1u : 0u);
                         flags |= kIsFew | (qslot ? kQSlot1 : 0) | (i + 1 == steps ? kFreeQ : 0);
                     } else {
+                        if (leader)
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            mma_ss(leader, tm + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
+                            mma_f16_ss(tm + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
                                        kk > 0 ? 1u : 0u);
                     }
                     commit(leader, bar_s + t);
@@ -772,21 +755,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const uint32_t q_off = (flags & kQSlot1) ? G::kQSlotBytes : 0;
                         const uint64_t p0 = make_smem_desc(sb + q_off + G::kOffPt + t * G::kPtBytes, 16, 1024,
                                                      kLayoutSw128);
+                        if (leader)
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ss(leader, o_tm, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
+                            mma_f16_ss(o_tm, v0 + pg_vdelta<D>(kk), p0 + pt_delta(kk), idesc_vp,
                                        kk > 0 ? 1u : acc);
                         if (flags & kFreeQ) commit(leader, bar_qfree + ((flags & kQSlot1) ? 1 : 0));
                     } else {
+                        if (leader)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_ts(leader, o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
+                            mma_f16_ts(o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
                                        kk > 0 ? 1u : acc);
                         if (!wait(bar_p2 + t, phase)) return false;
                         tc_fence_after();
+                        if (leader)
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk)
-                            mma_ts(leader, o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
+                            mma_f16_ts(o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
                     }
                     if (flags & kLast) commit(leader, bar_o + t);
                     if (flags & kFreeV) {
@@ -805,8 +791,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // The other stream's O does not wait behind an S whose keys have
                     // not landed; and a segment of few rows ends with all its
                     // products, as the next one may need the query slot that holds P^T.
+                    // (Two tiles take twice the products per key: their loads are ahead.)
                     uint32_t other = (due >> (16 * (t ^ 1))) & 0xffffu;
-                    if (other != 0) {
+                    if (mode != kTwoTiles && other != 0) {
                         bool now = G::kHasFew && mode == kFew && i == steps;
 #pragma unroll 1
                         while (!now && i != steps && !__any_sync(0xffffffffu, mbar_test(full + ks, kph))) {
