@@ -1347,29 +1347,59 @@ struct JoinSmem {
     __align__(16) T tile[32][kJoinCols + 8];
 };
 
-// One partial into a lane's running maximum, sum and output.
-template <int D>
-__device__ __forceinline__ void join_part(const TcParams& p, int tile_row, int rows, int r, int col0, float& top,
-                                          float& tot, float4 (&acc)[kJoinCols / 4]) {
-    constexpr int Q = kJoinCols / 4;
-    const float lse = p.L_part[tile_row + r];
-    const float4* src = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(tile_row) * D) +
-                        (col0 / 4) * rows + r;
-    float4 v[Q];
+// A lane's running maximum, sum and output, and two partials into it (their
+// loads in flight together; the second may be absent).
+struct JoinState {
+    float top, tot;
+    float4 acc[kJoinCols / 4];
+};
+
+__device__ __forceinline__ void join_init(JoinState& st) {
+    st.top = -INFINITY;
+    st.tot = 0.f;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) v[q] = src[q * rows];
-    const float m = fmaxf(top, lse);
-    const float m0 = m == -INFINITY ? 0.f : m;
-    const float w0 = sm100::ex2_approx(top - m0), w1 = sm100::ex2_approx(lse - m0);
-    top = m;
-    tot = tot * w0 + w1;
+    for (int q = 0; q < kJoinCols / 4; ++q) st.acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+struct PartRow {
+    int tile_row, rows, r;
+};
+
+template <int D>
+__device__ __forceinline__ void join_two(const TcParams& p, JoinState& st, const PartRow& a, const PartRow& b,
+                                         bool has_b, int col0) {
+    constexpr int Q = kJoinCols / 4;
+    const float4* src0 = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(a.tile_row) * D) +
+                         (col0 / 4) * a.rows + a.r;
+    const float4* src1 = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(b.tile_row) * D) +
+                         (col0 / 4) * b.rows + b.r;
+    float4 v0[Q], v1[Q];
+    const float l0 = p.L_part[a.tile_row + a.r];
+    const float l1 = has_b ? p.L_part[b.tile_row + b.r] : -INFINITY;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        acc[q].x = fmaf(w1, v[q].x, acc[q].x * w0);
-        acc[q].y = fmaf(w1, v[q].y, acc[q].y * w0);
-        acc[q].z = fmaf(w1, v[q].z, acc[q].z * w0);
-        acc[q].w = fmaf(w1, v[q].w, acc[q].w * w0);
+        v0[q] = src0[q * a.rows];
+        v1[q] = has_b ? src1[q * b.rows] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    const float m = fmaxf(fmaxf(st.top, l0), l1);
+    const float m0 = m == -INFINITY ? 0.f : m;
+    const float w = sm100::ex2_approx(st.top - m0);
+    const float w0 = sm100::ex2_approx(l0 - m0), w1 = sm100::ex2_approx(l1 - m0);
+    st.top = m;
+    st.tot = st.tot * w + (w0 + w1);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        st.acc[q].x = fmaf(w1, v1[q].x, fmaf(w0, v0[q].x, st.acc[q].x * w));
+        st.acc[q].y = fmaf(w1, v1[q].y, fmaf(w0, v0[q].y, st.acc[q].y * w));
+        st.acc[q].z = fmaf(w1, v1[q].z, fmaf(w0, v0[q].z, st.acc[q].z * w));
+        st.acc[q].w = fmaf(w1, v1[q].w, fmaf(w0, v0[q].w, st.acc[q].w * w));
+    }
+}
+
+// Partial k of two lists, one behind the other.
+__device__ __forceinline__ PartRow part_row(const Parts& a, const Parts& b, int k) {
+    return k < a.n ? PartRow{a.base + k * a.step, a.rows, a.r}
+                   : PartRow{b.base + (k - a.n) * b.step, b.rows, b.r};
 }
 
 // Joins the partials of both lists, a lane's row going to out_row (-1: none),
@@ -1380,22 +1410,16 @@ __device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, co
     constexpr int Q = kJoinCols / 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = a.n + b.n;
-    float4 acc[Q];
-    float top = -INFINITY, tot = 0.f;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    JoinState st;
+    join_init(st);
 #pragma unroll 1
-    for (int k = warp; k < n; k += kJoinWarps) {
-        const bool in_a = k < a.n;
-        const int at = in_a ? a.base + k * a.step : b.base + (k - a.n) * b.step;
-        const int r = in_a ? a.r : b.r, rows = in_a ? a.rows : b.rows;
-        join_part<D>(p, at, rows, r, col0, top, tot, acc);
-    }
+    for (int k = warp; k < n; k += 2 * kJoinWarps)
+        join_two<D>(p, st, part_row(a, b, k), part_row(a, b, min(k + kJoinWarps, n - 1)), k + kJoinWarps < n, col0);
     __syncthreads();  // the last use of the shared memory is over
 #pragma unroll
-    for (int q = 0; q < Q; ++q) sm.acc[warp][q][lane] = acc[q];
-    sm.top[warp][lane] = top;
-    sm.tot[warp][lane] = tot;
+    for (int q = 0; q < Q; ++q) sm.acc[warp][q][lane] = st.acc[q];
+    sm.top[warp][lane] = st.top;
+    sm.tot[warp][lane] = st.tot;
     if (warp == 0) sm.row[lane] = out_row;
     __syncthreads();
     // warp q: columns 4 q .. 4 q + 3
@@ -1404,7 +1428,7 @@ __device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, co
     for (int u = 0; u < kJoinWarps; ++u) M = fmaxf(M, sm.top[u][lane]);
     const float M0 = M == -INFINITY ? 0.f : M;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    tot = 0.f;
+    float tot = 0.f;
 #pragma unroll
     for (int u = 0; u < kJoinWarps; ++u) {
         const float w = sm100::ex2_approx(sm.top[u][lane] - M0);
@@ -1488,23 +1512,22 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int n_rec = 2 * ln.pieces;
     const int run = (n_rec + kJoinThreads - 1) / kJoinThreads;
     auto piece_of = [&](int i) -> int { return i < ln.pieces ? i : i - ln.pieces; };
-    // items of record i: groups of 32 rows times groups of columns
-    auto items = [&](int i, int kind) -> int {
+    // items of record i (light in the low half, heavy in the high half): groups of
+    // 32 rows times groups of columns
+    auto items = [&](int i) -> unsigned {
         if (i >= n_rec) return 0;
         const Split sp = ln.split[i];
         const int n = sp.last - piece_of(i) + 1;
-        if (n <= 1 || (n > kLightParts) != (kind == 1)) return 0;
+        if (n <= 1) return 0;
         const int tokens = min(sp.tok_end - sp.tok0, sp.mode == kTwoTiles ? 2 * ln.tpt : ln.tpt);
         const int rows = tokens > ln.tpt ? kTileRows + (tokens - ln.tpt) * ln.gt : tokens * ln.gt;
-        return (rows + 31) / 32 * kColGroups;
+        return static_cast<unsigned>((rows + 31) / 32 * kColGroups) << (n > kLightParts ? 16 : 0);
     };
+    unsigned mine = 0;
 #pragma unroll 1
-    for (int kind = 0; kind < 2; ++kind) {
-        int mine = 0;
-#pragma unroll 1
-        for (int k = 0; k < run; ++k) mine += items(threadIdx.x * run + k, kind);
-        ends[kind][threadIdx.x + 1] = mine;
-    }
+    for (int k = 0; k < run; ++k) mine += items(threadIdx.x * run + k);
+    ends[0][threadIdx.x + 1] = mine & 0xffffu;
+    ends[1][threadIdx.x + 1] = mine >> 16;
     __syncthreads();
     if (warp < 2) {  // inclusive sums, 8 threads' counts per lane
         int v[kJoinThreads / 32], sum = 0;
@@ -1539,11 +1562,12 @@ __global__ void __launch_bounds__(kJoinThreads)
             if (hit != 0) owner = k * 32 + __ffs(hit) - 1;
         }
         int left = at - ends[kind][owner], rec = owner * run;
-        int n = items(rec, kind);
+        auto of_kind = [&](unsigned v) -> int { return static_cast<int>(kind ? v >> 16 : v & 0xffffu); };
+        int n = of_kind(items(rec));
 #pragma unroll 1
         while (left >= n) {
             left -= n;
-            n = items(++rec, kind);
+            n = of_kind(items(++rec));
         }
         const Split sp = ln.split[rec];
         const bool few = rec >= ln.pieces;
@@ -1570,32 +1594,29 @@ __global__ void __launch_bounds__(kJoinThreads)
         join_rows<T, D>(p, sm, it.head, it.rest, it.out_row, it.col0);
     }
 #pragma unroll 1
-    for (int at = blockIdx.x * kJoinWarps + warp; at < light; at += gridDim.x * kJoinWarps) {
+    for (int at = (gridDim.x - 1 - blockIdx.x) * kJoinWarps + warp; at < light; at += gridDim.x * kJoinWarps) {
         const Item it = find(at, 0);
         if (it.out_row < 0) continue;
         constexpr int Q = kJoinCols / 4;
-        float4 acc[Q];
-        float top = -INFINITY, tot = 0.f;
-#pragma unroll
-        for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        JoinState st;
+        join_init(st);
         const int n = it.rest.n + 1;
 #pragma unroll 1
-        for (int k = 0; k < n; ++k) {
-            const int tile_row = k == 0 ? it.head.base : it.rest.base + (k - 1) * it.rest.step;
-            join_part<D>(p, tile_row, it.head.rows, it.head.r, it.col0, top, tot, acc);
-        }
-        const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
+        for (int k = 0; k < n; k += 2)
+            join_two<D>(p, st, part_row(it.head, it.rest, k), part_row(it.head, it.rest, min(k + 1, n - 1)),
+                        k + 1 < n, it.col0);
+        const float inv = st.tot > 0.f ? __fdividef(1.f, st.tot) : 0.f;
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(it.out_row) * D + it.col0);
 #pragma unroll
         for (int q = 0; q < Q; q += 2) {
             uint4 v;
-            v.x = DType<T>::pack2(acc[q].x * inv, acc[q].y * inv);
-            v.y = DType<T>::pack2(acc[q].z * inv, acc[q].w * inv);
-            v.z = DType<T>::pack2(acc[q + 1].x * inv, acc[q + 1].y * inv);
-            v.w = DType<T>::pack2(acc[q + 1].z * inv, acc[q + 1].w * inv);
+            v.x = DType<T>::pack2(st.acc[q].x * inv, st.acc[q].y * inv);
+            v.y = DType<T>::pack2(st.acc[q].z * inv, st.acc[q].w * inv);
+            v.z = DType<T>::pack2(st.acc[q + 1].x * inv, st.acc[q + 1].y * inv);
+            v.w = DType<T>::pack2(st.acc[q + 1].z * inv, st.acc[q + 1].w * inv);
             dst[q / 2] = v;
         }
-        if (it.col0 == 0) p.L[it.out_row] = tot > 0.f ? (top + __log2f(tot)) * kLn2 : -INFINITY;
+        if (it.col0 == 0) p.L[it.out_row] = st.tot > 0.f ? (st.top + __log2f(st.tot)) * kLn2 : -INFINITY;
     }
 }
 
