@@ -659,6 +659,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ok = __all_sync(0xffffffffu, poll(bar, parity));
                     return ok;
                 };
+                // two at once: their first tries, usually successful, overlap
+                auto wait2 = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) -> bool {
+                    const bool ra = mbar_try_wait(smem_u32(a), pa), rb = mbar_try_wait(smem_u32(b), pb);
+                    ok = __all_sync(0xffffffffu, (ra || poll(a, pa)) && (rb || poll(b, pb)));
+                    return ok;
+                };
                 constexpr uint32_t idesc_qk = make_idesc(DType<T>::kMmaFmt, 128, 128, false, false);
                 constexpr uint32_t idesc_pv = make_idesc(DType<T>::kMmaFmt, 128, D, false, true);
                 constexpr uint32_t idesc_kq = make_idesc(DType<T>::kMmaFmt, 128, kFewRows, false, false);
@@ -673,6 +679,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 int k = 0, qs = 0, cur_q = 0;
                 int i = 0, steps = 0, mode = kTwoTiles;
                 bool end = false;
+                bool k_ready = false;  // the next K fill is known to have landed
                 auto next_slot = [](uint32_t& s, uint32_t& ph) {
                     s += 2;
                     if (s >= R) {
@@ -707,7 +714,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     const bool two = mode == kTwoTiles;
                     const int u = two ? i & 1 : 0;
-                    if (u == 0 && !wait(full + ks, kph)) return 0;
+                    if (u == 0 && !k_ready && !wait(full + ks, kph)) return 0;
+                    k_ready = false;
                     const int qslot = two ? u : cur_q;
                     tc_fence_after();
                     const uint64_t a0 = pg_kdesc<D>(sb + qslot * G::kQSlotBytes);
@@ -745,8 +753,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // O of stream t's step, in step order
                 auto issue_o = [&](int t, uint32_t flags) -> bool {
                     const uint32_t phase = (par >> t) & 1;
-                    if ((flags & kWaitV) && !wait(full + vs, vph)) return false;
-                    if (!wait(bar_p + t, phase)) return false;
+                    if (flags & kWaitV) {
+                        if (!wait2(full + vs, vph, bar_p + t, phase)) return false;
+                    } else if (!wait(bar_p + t, phase)) {
+                        return false;
+                    }
                     const uint64_t v0 = pg_vdesc<D>(sb + G::kOffRing + vs * G::kTileBytes);
                     const uint32_t o_tm = tm + 256 + t * 128;
                     const uint32_t acc = (flags & kAcc) ? 1u : 0u;
@@ -767,7 +778,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int kk = 0; kk < 4; ++kk)
                             mma_f16_ts(o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
                                        kk > 0 ? 1u : acc);
+                        const bool kr = mbar_test(full + ks, kph);
                         if (!wait(bar_p2 + t, phase)) return false;
+                        k_ready = __all_sync(0xffffffffu, kr);
                         tc_fence_after();
                         if (leader)
 #pragma unroll
