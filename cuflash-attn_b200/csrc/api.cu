@@ -372,7 +372,8 @@ FlashAttentionError kv_append_impl(const T* Q, const T* K, const T* V, T* Q_out,
                                    cudaStream_t stream) {
     if (!K || !V || !K_cache || !V_cache || !block_table || !seq_lens || !Q != !Q_out)
         return FlashAttentionError::NULL_POINTER;
-    if (num_tokens <= 0 || B <= 0 || Hkv <= 0 || D <= 0 || (Q && Hq <= 0))
+    if (num_tokens <= 0 || B <= 0 || Hkv <= 0 || D <= 0 || (Q && Hq <= 0) ||
+        2LL * Hkv + (Q ? Hq : 0) > 0x7fffffffLL)
         return FlashAttentionError::INVALID_DIMENSION;
     if (!paged_geometry_ok(page_size, max_pages, num_pages))
         return FlashAttentionError::INVALID_DIMENSION;

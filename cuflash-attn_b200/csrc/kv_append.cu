@@ -11,15 +11,17 @@
 // and value rows go to page block_table[b][p / page_size], slot
 // p % page_size; the queries to Q_out.
 //
-// Bound by bytes: each 16-bit element is read once and written once (2.9 kB
-// in and out per K/V pair of 8 heads of 128 and 32 query heads: 24.6 kB per
-// token), the angles' row (512 B in fp32) serves every head of the token.  A
-// block of 128 threads takes one token; a thread owns the same 16 bytes
-// (8 elements) of every head it visits, so the angles it needs stay in
-// registers, and it issues the loads of all its heads before it looks up the
-// token's sequence, so that the dependent look-ups (sequence, length, page)
-// overlap them.  The partner of an element is half a rotation away in the
-// same head and is fetched from the owning lane by a shuffle.
+// Bound by bytes: each 16-bit element is read once and written once (24.6 kB
+// per token of 32 query heads and 8 key/value heads of 128), the angles' row
+// (512 B in fp32) serves every head of the token.  A block of 128 threads takes
+// one token; a thread owns the same 16 bytes (8 elements) of every head it
+// visits, so the angles it needs stay in registers, and it issues the loads of
+// all its heads before it looks up the token's sequence, so that the dependent
+// look-ups (sequence, length, page) overlap them.  The partner of an element
+// is half a rotation away in the same head and is fetched from the owning lane
+// by a shuffle.  Measured, at those sizes: 26915 tokens in 124 us (5.4 TB/s of
+// elements, 0.84 of a plain copy's rate); 256 tokens in 4.1 us inside a graph,
+// which is the launch and the chain of look-ups.
 
 #include "common.cuh"
 #include "paged.cuh"

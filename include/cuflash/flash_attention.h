@@ -283,6 +283,16 @@ CUFLASH_EXPORT int cuflash_kv_append_paged_f16(
 // no key gets O = 0 and L = -inf; rows from cu_seqlens[B] on are left as they
 // were.  Sequences may have any number of new tokens, none included, so one
 // call serves prompts, chunks of prompts and single tokens together.
+//
+// For both attention entries: Q, the cache and O are 16-byte aligned (else
+// CUDA_ERROR).  Cache rows behind a sequence's length may hold anything, NaN
+// included.  Keys that causality hides from a row have weight zero in it, so
+// their value rows must be finite (0 * NaN).  Results are reproducible bit by
+// bit: how the work is divided depends on the lengths and the device, and
+// nothing is summed by atomics.  Pages of 8 rows and more run on the tensor
+// cores; smaller ones take a kernel that reads the keys once per query head
+// and token.  INVALID_DIMENSION also where num_tokens * num_q_heads or the
+// partial results of a call would pass 2^31 rows.
 CUFLASH_EXPORT int cuflash_attention_forward_paged_bf16(
     const __nv_bfloat16* Q, const __nv_bfloat16* K_cache, const __nv_bfloat16* V_cache,
     const int* block_table, const int* seq_lens, const int* cu_seqlens, __nv_bfloat16* O, float* L,

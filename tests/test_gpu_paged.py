@@ -322,6 +322,111 @@ def test_forward_paged_matches_dense_forward(lib, cuda):
     assert float((L - L2[0].transpose(0, 1)).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("group", [1, 2, 3, 8, 15, 16, 17, 40])
+@pytest.mark.parametrize("D", [64, 128])
+def test_forward_paged_few_rows(lib, cuda, group, D):
+    """One to four new tokens per sequence over short and long histories: the
+    forms of few rows, their borders to the row tiles, keys split over CTAs."""
+    new = [1, 1, 2, 1, 4, 3, 1, 1, 5]
+    lens = [3000, 1, 129, 5, 700, 3, 0, 6500, 260]
+    _check_forward(lib, new, lens, 2 * group, 2, D, 16, "bf16", True, seed=31)
+    _check_forward(lib, new, lens, group, 1, D, 64, "f16", False, seed=32)
+
+
+def test_forward_paged_many_sequences(lib, cuda):
+    """More sequences than threads of a CTA, the kinds of units mixed."""
+    new = [(b % 5 == 0) * (1 + b % 9) for b in range(1300)]
+    lens = [(n > 0) * (n + (17 * b) % 41) for b, n in enumerate(new)]
+    _check_forward(lib, new, lens, 4, 2, 64, 8, "bf16", True, seed=33, tail=5)
+
+
+@pytest.mark.parametrize("page_size", [2, 16])
+@pytest.mark.parametrize("D", [32, 128])
+def test_forward_paged_not_a_number(lib, cuda, page_size, D):
+    """A NaN in a key that rows see makes those rows' O and L NaN, and no other
+    row's; in a key that causality hides from a row it leaves the row alone.  A
+    NaN in a value reaches O only."""
+    import torch
+
+    new, lens = [3, 1, 140, 1], [30, 200, 150, 400]
+    c = Cache(lens, page_size, 2, D, torch.bfloat16, 34)
+    q = _randn(c.gen, sum(new), 4, D, dtype=torch.bfloat16)
+    args = (c.table, _i32(lens), _cu(new))
+    want, want_l = lib.forward_paged(q, c.K, c.V, *args)
+    nan = float("nan")
+    K = c.K.clone()
+    K.view(-1, 2, D)[c.rows(0, 30)[28], 0, 1] = nan    # hidden from token 0 of sequence 0
+    K.view(-1, 2, D)[c.rows(1, 200)[77], 1, 0] = nan
+    K.view(-1, 2, D)[c.rows(2, 150)[149], 0, 3] = nan  # seen by the last token alone
+    O, L = lib.forward_paged(q, K, c.V, *args)
+    hit = torch.zeros((sum(new), 4), dtype=torch.bool, device="cuda")
+    hit[1:3, :2] = True
+    hit[3, 2:] = True
+    hit[143, :2] = True
+    assert torch.equal(torch.isnan(L), hit)
+    assert torch.equal(torch.isnan(O).all(-1), hit) and torch.equal(torch.isnan(O).any(-1), hit)
+    assert torch.equal(O[~hit], want[~hit]) and torch.equal(L[~hit], want_l[~hit])
+    V = c.V.clone()
+    V.view(-1, 2, D)[c.rows(3, 400)[300], 0, 5] = nan
+    O, L = lib.forward_paged(q, c.K, V, *args)
+    assert torch.equal(L, want_l) and bool(torch.isnan(O[144, :2, 5]).all())
+    O[144, :2, 5] = want[144, :2, 5]
+    assert torch.equal(O, want)
+    # the same through the prefix decode: prefix 0's keys, own keys of 1 and 3
+    qd = q[:2].unsqueeze(2).contiguous()
+    own = c.table[[1, 3]].contiguous()
+    O, L = lib.decode_shared_prefix(qd, K, c.V, c.table[2], _i32([140]), own, _i32([200, 400]))
+    hit = torch.tensor([[False, False, True, True], [False] * 4], device="cuda")
+    assert torch.equal(torch.isnan(L), hit) and torch.equal(torch.isnan(O).any(-1)[..., 0], hit)
+    O, L = lib.decode_shared_prefix(qd, K, c.V, c.table[2], _i32([150]), own, _i32([200, 400]))
+    hit[:, :2] = True
+    assert torch.equal(torch.isnan(L), hit) and torch.equal(torch.isnan(O).any(-1)[..., 0], hit)
+
+
+@pytest.mark.parametrize("page_size", [4, 32])
+def test_lengths_and_pages_out_of_range(lib, cuda, page_size):
+    """Lengths beyond the table count as the table's, negative ones as zero; a
+    page outside the pool gives some page's rows and touches nothing else."""
+    import torch
+
+    new, lens = [2, 1, 9, 1], [128, 96, 128, 60]
+    c = Cache(lens, page_size, 1, 64, torch.bfloat16, 35)
+    q = _randn(c.gen, sum(new), 4, 64, dtype=torch.bfloat16)
+    want = lib.forward_paged(q, c.K, c.V, c.table, _i32(lens), _cu(new))
+    far = lib.forward_paged(q, c.K, c.V, c.table, _i32([1 << 30, 96, 1 << 20, 60]), _cu(new))
+    for x, y in zip(want, far):
+        assert torch.equal(x, y)
+    O, L = lib.forward_paged(q, c.K, c.V, c.table, _i32([128, -5, 128, 60]), _cu(new))
+    assert bool((O[2] == 0).all()) and bool(torch.isneginf(L[2]).all())
+    rest = [0, 1] + list(range(3, 13))
+    assert torch.equal(O[rest], want[0][rest]) and torch.equal(L[rest], want[1][rest])
+    bad = c.table.clone()
+    bad[1, 1], bad[3, 0] = -3, c.num_pages + 1000
+    O, L = lib.forward_paged(q, c.K, c.V, bad, _i32(lens), _cu(new))
+    rest = [0, 1] + list(range(3, 12))
+    assert torch.equal(O[rest], want[0][rest]) and torch.equal(L[rest], want[1][rest])
+    assert lib.device_status() == 0
+
+
+def test_sequences_that_share_pages(lib, cuda):
+    """The same pages in several rows of the table, and twice in one."""
+    import torch
+
+    c = Cache([200], 16, 2, 128, torch.bfloat16, 36)
+    row = c.table[0].clone()
+    row[5] = row[4]
+    table = torch.stack([c.table[0], c.table[0], row])
+    q = _randn(c.gen, 3, 8, 128, dtype=torch.bfloat16)
+    q[1] = q[0]
+    O, L = lib.forward_paged(q, c.K, c.V, table, _i32([200] * 3), _cu([1] * 3))
+    assert torch.equal(O[0], O[1]) and torch.equal(L[0], L[1])
+    r = ref.cache_rows(row, torch.arange(200, device="cuda"), 16)
+    k, v = c.K.view(-1, 2, 128)[r], c.V.view(-1, 2, 128)[r]
+    O64, L64, bO, bL = ref.attend(q[2:], k, v, 128 ** -0.5, None, torch.bfloat16)
+    ref.check(O[2:], O64, bO, "O")
+    ref.check(L[2:], L64, bL, "L")
+
+
 # ----------------------------------------------------- shared-prefix decode
 def _check_prefix(lib, prefix, lens, Hq, Hkv, D, page_size, dt, seed=0, ramp=None):
     import torch
@@ -373,6 +478,11 @@ def test_shared_prefix_long(lib, cuda):
 def test_shared_prefix_wide_groups(lib, cuda):
     _check_prefix(lib, 333, [5, 0, 140], 160, 1, 64, 16, "bf16", seed=14)
     _check_prefix(lib, 200, [9, 150], 256, 2, 32, 8, "f16", seed=15)
+
+
+@pytest.mark.parametrize("group", [1, 8, 16, 17])
+def test_shared_prefix_groups(lib, cuda, group):
+    _check_prefix(lib, 1500, [900, 0, 3, 129, 5000], 2 * group, 2, 128, 16, "bf16", seed=17)
 
 
 def test_shared_prefix_no_key_at_all(lib, cuda):
@@ -548,6 +658,20 @@ def test_two_streams_at_once(lib, cuda):
         torch.cuda.synchronize()
         for (O, L), (O2, L2) in zip(got, want):
             assert torch.equal(O, O2) and torch.equal(L, L2)
+
+
+@pytest.mark.parametrize("reserve", [1, 147])
+def test_reserved_sms(lib, cuda, reserve):
+    """Fewer CTAs cut the work into fewer pieces."""
+    import cuflash_attn as cf
+
+    option = lib.lib.cuflash_set_option
+    assert option(b"CUFLASH_RESERVE_SMS", reserve) == cf.SUCCESS
+    try:
+        _check_forward(lib, [1, 300, 1, 7], [900, 1000, 40, 7], 8, 2, 64, 16, "bf16", True, seed=25)
+        _check_prefix(lib, 700, [5, 0, 400], 8, 2, 64, 16, "bf16", seed=26)
+    finally:
+        assert option(b"CUFLASH_RESERVE_SMS", -1) == cf.SUCCESS
 
 
 def test_offsets_beyond_32_bits(lib, cuda):

@@ -52,6 +52,7 @@ APPEND = [
     (dict(qs=128), cf.INVALID_DIMENSION), (dict(qs=260), cf.INVALID_DIMENSION),
     (dict(ks=64), cf.INVALID_DIMENSION), (dict(vs=-128), cf.INVALID_DIMENSION),
     (dict(qs=512), cf.INVALID_DIMENSION),  # in place (Q == Q_out) but not contiguous
+    (dict(Hkv=1 << 30), cf.INVALID_DIMENSION),
     (dict(K=ctypes.c_void_p(0x1008)), cf.CUDA_ERROR),  # 16-byte alignment
 ]
 
