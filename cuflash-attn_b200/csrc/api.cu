@@ -769,6 +769,34 @@ int cuflash_attention_decode_bf16_noalloc(const __nv_bfloat16* Q, const __nv_bfl
             true, Q, K_cache, V_cache, prefix_table, prefix_len, block_table, seq_lens, nullptr,   \
             O, L, batch_size, batch_size, num_q_heads, num_kv_heads, head_dim, page_size,          \
             max_prefix_pages, max_pages_per_seq, num_pages, scale, false, stream));                \
+    }                                                                                              \
+    int cuflash_kv_append_paged_args_##SUFFIX(const CuflashKvAppendArgs* a) {                      \
+        if (a == nullptr) return static_cast<int>(FlashAttentionError::NULL_POINTER);              \
+        return static_cast<int>(kv_append_impl<T>(                                                 \
+            static_cast<const T*>(a->Q), static_cast<const T*>(a->K), static_cast<const T*>(a->V), \
+            static_cast<T*>(a->Q_out), static_cast<T*>(a->K_cache), static_cast<T*>(a->V_cache),   \
+            a->rope_table, a->positions, a->block_table, a->seq_lens, a->cu_seqlens,               \
+            a->num_tokens, a->batch_size, a->num_q_heads, a->num_kv_heads, a->head_dim,            \
+            a->page_size, a->max_pages_per_seq, a->num_pages, a->q_stride, a->k_stride,            \
+            a->v_stride, a->rotary_dim, a->max_position, a->interleaved != 0, a->stream));         \
+    }                                                                                              \
+    int cuflash_attention_forward_paged_args_##SUFFIX(const CuflashPagedAttentionArgs* a) {        \
+        if (a == nullptr) return static_cast<int>(FlashAttentionError::NULL_POINTER);              \
+        return cuflash_attention_forward_paged_##SUFFIX(                                           \
+            static_cast<const T*>(a->Q), static_cast<const T*>(a->K_cache),                        \
+            static_cast<const T*>(a->V_cache), a->block_table, a->seq_lens, a->cu_seqlens,         \
+            static_cast<T*>(a->O), a->L, a->num_tokens, a->batch_size, a->num_q_heads,             \
+            a->num_kv_heads, a->head_dim, a->page_size, a->max_pages_per_seq, a->num_pages,        \
+            a->scale, a->causal != 0, a->stream);                                                  \
+    }                                                                                              \
+    int cuflash_attention_decode_shared_prefix_args_##SUFFIX(const CuflashPagedAttentionArgs* a) { \
+        if (a == nullptr) return static_cast<int>(FlashAttentionError::NULL_POINTER);              \
+        return cuflash_attention_decode_shared_prefix_##SUFFIX(                                    \
+            static_cast<const T*>(a->Q), static_cast<const T*>(a->K_cache),                        \
+            static_cast<const T*>(a->V_cache), a->prefix_table, a->prefix_len, a->block_table,     \
+            a->seq_lens, static_cast<T*>(a->O), a->L, a->batch_size, a->num_q_heads,               \
+            a->num_kv_heads, a->head_dim, a->page_size, a->max_prefix_pages,                       \
+            a->max_pages_per_seq, a->num_pages, a->scale, a->stream);                              \
     }
 CUFLASH_PAGED_ENTRIES(bf16, __nv_bfloat16)
 CUFLASH_PAGED_ENTRIES(f16, half)

@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from pathlib import Path
 from typing import Optional, Tuple
 
@@ -65,6 +66,13 @@ SIGNATURES = {
     "cuflash_attention_forward_paged_f16": [_P] * 8 + [_I] * 8 + [_F, _B, _P],
     "cuflash_attention_decode_shared_prefix_bf16": [_P] * 9 + [_I] * 8 + [_F, _P],
     "cuflash_attention_decode_shared_prefix_f16": [_P] * 9 + [_I] * 8 + [_F, _P],
+    # with their arguments packed (PAGED_ARGS)
+    "cuflash_kv_append_paged_args_bf16": [ctypes.c_char_p],
+    "cuflash_kv_append_paged_args_f16": [ctypes.c_char_p],
+    "cuflash_attention_forward_paged_args_bf16": [ctypes.c_char_p],
+    "cuflash_attention_forward_paged_args_f16": [ctypes.c_char_p],
+    "cuflash_attention_decode_shared_prefix_args_bf16": [ctypes.c_char_p],
+    "cuflash_attention_decode_shared_prefix_args_f16": [ctypes.c_char_p],
     "cuflash_attention_forward_gqa_bf16": [_P] * 5 + [_I] * 6 + [_F, _B, _P],
     "cuflash_attention_forward_gqa_f16": [_P] * 5 + [_I] * 6 + [_F, _B, _P],
     "cuflash_attention_backward_gqa_bf16": [_P] * 9 + [_I] * 6 + [_F, _B, _P],
@@ -91,6 +99,9 @@ SIGNATURES = {
     "cuflash_profile_main_kernels": [_I],
     "cuflash_profile_read_ms": [_P, _I],
 }
+# CuflashKvAppendArgs and CuflashPagedAttentionArgs, in the header's order
+APPEND_ARGS = struct.Struct("@11P3q11iP")
+PAGED_ARGS = struct.Struct("@10P10ifP")
 _RESTYPES = {"cuflash_error_string": ctypes.c_char_p,
              "cuflash_attention_backward_cp_workspace_size": ctypes.c_longlong}
 
@@ -244,18 +255,18 @@ class CuFlashAttn:
             fn = self._paged_fn[key] = getattr(self.lib, f"{entry}_{_suffix(t)}")
         return fn
 
-    def _call_on(self, device: int, stream, fn, *args) -> None:
-        """fn(*args, stream) with `device` current; by default on its current
-        stream."""
+    def _call_on(self, device: int, stream, fn, pack, *args) -> None:
+        """fn(pack(*args, stream)) with `device` current; by default on its
+        current stream."""
         import torch
 
         raw = (torch._C._cuda_getCurrentRawStream(device) if stream is None
                else stream.cuda_stream)
         if torch._C._cuda_getDevice() == device:
-            code = fn(*args, raw)
+            code = fn(pack(*args, raw))
         else:
             with torch.cuda.device(device):
-                code = fn(*args, raw)
+                code = fn(pack(*args, raw))
         if code:
             self.check_error(code)
 
@@ -431,11 +442,12 @@ class CuFlashAttn:
                 _require(device, (torch.float32, {"rope_table": rope_table}))
             max_position, rotary = rope_table.shape
             rope_ptr = rope_table.data_ptr()
-        self._call_on(device, stream, self._paged("cuflash_kv_append_paged", K), q_ptr,
-                      K.data_ptr(), V.data_ptr(), out_ptr, K_cache.data_ptr(),
-                      V_cache.data_ptr(), rope_ptr, pos_ptr, block_table.data_ptr(),
-                      seq_lens.data_ptr(), cu_ptr, tokens, B, Hq, Hkv, D, page_size, max_pages,
-                      num_pages, q_stride, k_stride, v_stride, rotary, max_position, interleaved)
+        self._call_on(device, stream, self._paged("cuflash_kv_append_paged_args", K),
+                      APPEND_ARGS.pack, q_ptr, K.data_ptr(), V.data_ptr(), out_ptr,
+                      K_cache.data_ptr(), V_cache.data_ptr(), rope_ptr, pos_ptr,
+                      block_table.data_ptr(), seq_lens.data_ptr(), cu_ptr, q_stride, k_stride,
+                      v_stride, tokens, B, Hq, Hkv, D, page_size, max_pages, num_pages, rotary,
+                      max_position, bool(interleaved))
         return Q_out
 
     def forward_paged(self, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens,
@@ -464,11 +476,11 @@ class CuFlashAttn:
                      (torch.int32, {"block_table": block_table, "seq_lens": seq_lens,
                                     "cu_seqlens": cu_seqlens}))
         O, L = self._outputs(Q, device, shape, (tokens, Hq), O, L)
-        self._call_on(device, stream, self._paged("cuflash_attention_forward_paged", Q),
-                      Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
+        self._call_on(device, stream, self._paged("cuflash_attention_forward_paged_args", Q),
+                      PAGED_ARGS.pack, Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), 0, 0,
                       block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-                      O.data_ptr(), L.data_ptr(), tokens, B, Hq, Hkv, D, page_size, max_pages,
-                      num_pages, D ** -0.5 if scale is None else scale, causal)
+                      O.data_ptr(), L.data_ptr(), tokens, B, Hq, Hkv, D, page_size, 0, max_pages,
+                      num_pages, bool(causal), D ** -0.5 if scale is None else scale)
         return O, L
 
     def decode_shared_prefix(self, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
@@ -504,11 +516,13 @@ class CuFlashAttn:
                      (torch.int32, {"prefix_table": prefix_table, "prefix_len": prefix_len,
                                     "block_table": block_table, "seq_lens": seq_lens}))
         O, L = self._outputs(q, device, shape, (B, Hq), O, L)
-        self._call_on(device, stream, self._paged("cuflash_attention_decode_shared_prefix", q),
-                      q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
+        self._call_on(device, stream,
+                      self._paged("cuflash_attention_decode_shared_prefix_args", q),
+                      PAGED_ARGS.pack, q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
                       prefix_table.data_ptr(), prefix_len.data_ptr(), block_table.data_ptr(),
-                      seq_lens.data_ptr(), O.data_ptr(), L.data_ptr(), B, Hq, Hkv, D, page_size,
-                      max_prefix, max_pages, num_pages, D ** -0.5 if scale is None else scale)
+                      seq_lens.data_ptr(), 0, O.data_ptr(), L.data_ptr(), B, B, Hq, Hkv, D,
+                      page_size, max_prefix, max_pages, num_pages, False,
+                      D ** -0.5 if scale is None else scale)
         return O, L
 
     @staticmethod

@@ -641,6 +641,56 @@ def test_captured_step_follows_lengths(lib, cuda):
     assert lib.device_status() == 0
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_entries_with_single_arguments(lib, cuda, dt):
+    """The C entries that take their arguments one by one do what the binding's
+    packed ones do."""
+    import torch
+
+    dtype, Hq, Hkv, D, ps = _dtype(dt), 8, 2, 64, 16
+    new, lens, T = [3, 1, 20], [40, 7, 150], 24
+    packed, single = (Cache(lens, ps, Hkv, D, dtype, 27) for _ in range(2))
+    qkv = _randn(packed.gen, T, Hq + 2 * Hkv, D, dtype=dtype)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]
+    rope = torch.randn(160, 32, device="cuda")
+    cu, sl = _cu(new), _i32(lens)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") * 5
+
+    def ptr(t):
+        return t.data_ptr()
+
+    def call(entry, *args):
+        stream = torch.cuda.current_stream().cuda_stream
+        assert getattr(lib.lib, f"cuflash_{entry}_{dt}")(*args, stream) == 0
+
+    want_q = lib.kv_append_paged(k, v, packed.K, packed.V, packed.table, sl, cu, Q=q,
+                                 rope_table=rope, positions=pos, interleaved=True)
+    got_q, c = torch.empty_like(want_q), single
+    row = (Hq + 2 * Hkv) * D
+    geometry = (ps, c.table.shape[1], c.num_pages)
+    call("kv_append_paged", ptr(q), ptr(k), ptr(v), ptr(got_q), ptr(c.K), ptr(c.V), ptr(rope),
+         ptr(pos), ptr(c.table), ptr(sl), ptr(cu), T, 3, Hq, Hkv, D, *geometry, row, row, row, 32,
+         160, True)
+    assert torch.equal(want_q, got_q)
+    for x, y in ((packed.K, c.K), (packed.V, c.V)):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+    want = lib.forward_paged(want_q, packed.K, packed.V, packed.table, sl, cu, causal=False,
+                             scale=0.2)
+    got = [torch.empty_like(x) for x in want]
+    call("attention_forward_paged", ptr(got_q), ptr(c.K), ptr(c.V), ptr(c.table), ptr(sl), ptr(cu),
+         ptr(got[0]), ptr(got[1]), T, 3, Hq, Hkv, D, *geometry, 0.2, False)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    qd, plen = want_q[:2].unsqueeze(2).contiguous(), _i32([40])
+    table, own = c.table[1:].contiguous(), _i32(lens[1:])
+    want = lib.decode_shared_prefix(qd, packed.K, packed.V, packed.table[0], plen, table, own,
+                                    scale=0.2)
+    got = [torch.empty_like(x) for x in want]
+    call("attention_decode_shared_prefix", ptr(qd), ptr(c.K), ptr(c.V), ptr(c.table[0]), ptr(plen),
+         ptr(table), ptr(own), ptr(got[0]), ptr(got[1]), 2, Hq, Hkv, D, ps, c.table.shape[1],
+         c.table.shape[1], c.num_pages, 0.2)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
 def test_two_streams_at_once(lib, cuda):
     """Calls on two streams whose kernels may overlap have their own workspaces."""
     import torch

@@ -98,6 +98,77 @@ def test_shared_prefix_refusals(lib, sfx, kw, code):
     assert _prefix(lib, sfx, **kw) == code
 
 
+def _ptr(x):
+    return x.value or 0 if isinstance(x, ctypes.c_void_p) else x
+
+
+class _Packed:
+    """The entries as their plain forms are called, through the packed ones."""
+
+    def __init__(self, lib):
+        self.raw, self.lib = lib.lib, self
+
+    def __getattr__(self, name):
+        entry, sfx = name.rsplit("_", 1)
+        fn = getattr(self.raw, f"{entry}_args_{sfx}")
+
+        def call(*a):
+            a = [_ptr(x) for x in a]
+            if entry == "cuflash_kv_append_paged":
+                return fn(cf.APPEND_ARGS.pack(*a[:11], *a[19:22], *a[11:19], *a[22:]))
+            if entry == "cuflash_attention_forward_paged":
+                return fn(cf.PAGED_ARGS.pack(*a[:3], 0, 0, *a[3:14], 0, *a[14:16], a[17], a[16],
+                                             a[18]))
+            return fn(cf.PAGED_ARGS.pack(*a[:7], 0, *a[7:9], a[9], *a[9:17], 0, *a[17:]))
+
+        return call
+
+
+@pytest.mark.parametrize("sfx", ["bf16", "f16"])
+def test_packed_arguments_refuse_alike(lib, sfx):
+    """Each field arrives in its place: every refusal, through the struct."""
+    packed = _Packed(lib)
+    for call, cases in ((_append, APPEND), (_forward, FORWARD), (_prefix, PREFIX)):
+        for kw, code in cases:
+            assert call(packed, sfx, **kw) == code, kw
+    for entry in ("kv_append_paged", "attention_forward_paged", "attention_decode_shared_prefix"):
+        assert getattr(lib.lib, f"cuflash_{entry}_args_{sfx}")(None) == cf.NULL_POINTER
+
+
+def test_packed_arguments_layout(tmp_path):
+    """The binding's formats have the sizes and offsets of the header's structs."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    cuda = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parents[1] / "include"
+    if not shutil.which("g++") or not (cuda / "cuda_runtime.h").exists():
+        pytest.skip("needs g++ and the CUDA headers")
+    src = tmp_path / "layout.cpp"
+    src.write_text("""
+#include <cstddef>
+#include <cstdio>
+#include "cuflash/flash_attention.h"
+#define AT(S, F) offsetof(S, F)
+int main() {
+    using A = CuflashKvAppendArgs;
+    using P = CuflashPagedAttentionArgs;
+    std::printf("%zu %zu %zu %zu %zu %zu %zu %zu", sizeof(A), AT(A, q_stride), AT(A, num_tokens),
+                AT(A, stream), sizeof(P), AT(P, num_tokens), AT(P, scale), AT(P, stream));
+}
+""")
+    exe = tmp_path / "layout"
+    subprocess.run(["g++", "-std=c++17", "-I", str(root / "include"), "-I", str(cuda), str(src),
+                    "-o", str(exe)], check=True)
+    import struct
+
+    got = [int(x) for x in subprocess.check_output([str(exe)]).split()]
+    a, p = cf.APPEND_ARGS, cf.PAGED_ARGS
+    assert got == [a.size, struct.calcsize("@11P"), struct.calcsize("@11P3q"), a.size - 8,
+                   p.size, struct.calcsize("@10P"), struct.calcsize("@10P10i"), p.size - 8]
+
+
 def test_binding_refuses_before_the_library(lib):
     """Shapes, types and devices are checked by the binding (CPU tensors)."""
     import torch
