@@ -74,6 +74,8 @@ __global__ void __launch_bounds__(kAppendThreads)
         if (h < p.hq + p.hkv) return p.K + t * p.k_stride + (h - p.hq) * D + c * 8;
         return p.V + t * p.v_stride + (h - p.hq - p.hkv) * D + c * 8;
     };
+    stream_release();
+    stream_wait();
     uint4 x[kAppendHeads];
 #pragma unroll
     for (int i = 0; i < kAppendHeads; ++i) {
@@ -188,12 +190,11 @@ __global__ void __launch_bounds__(kAppendThreads)
 template <typename T, int D>
 FlashAttentionError append_typed(const AppendParams<T>& p, int num_tokens, bool interleaved,
                                  cudaStream_t stream) {
-    if (interleaved)
-        kv_append_kernel<T, D, true><<<num_tokens, kAppendThreads, 0, stream>>>(p);
-    else
-        kv_append_kernel<T, D, false><<<num_tokens, kAppendThreads, 0, stream>>>(p);
-    return cudaGetLastError() == cudaSuccess ? FlashAttentionError::SUCCESS
-                                             : FlashAttentionError::CUDA_ERROR;
+    const cudaError_t err = launch_behind(interleaved ? kv_append_kernel<T, D, true>
+                                                      : kv_append_kernel<T, D, false>,
+                                          dim3(num_tokens), kAppendThreads, 0, stream, p);
+    if (err != cudaSuccess) cudaGetLastError();
+    return err == cudaSuccess ? FlashAttentionError::SUCCESS : FlashAttentionError::CUDA_ERROR;
 }
 
 }  // namespace

@@ -14,6 +14,33 @@ __host__ __device__ __forceinline__ int clamp_len(int n, int most) {
 }
 
 #ifdef __CUDACC__
+// Launches `kern` so that its blocks may be scheduled while the kernel before
+// it on the stream still runs: every thread calls stream_wait() before it
+// touches global memory, and none returns without.  Between calls of a serving
+// step this hides the launch and the set-up of a kernel.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_behind(void (*kern)(Params...), dim3 grid, int threads, size_t smem,
+                                 cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+__device__ __forceinline__ void stream_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// the next kernel's blocks may start; it waits for this one's end by itself
+__device__ __forceinline__ void stream_release() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // Sequence of token t among cu[0..B] (ascending, cu[b] = first token of
 // sequence b): the last b with cu[b] <= t < cu[b + 1], or -1 for a token
 // outside [cu[0], cu[B]).  Each round the 32 lanes probe 32 evenly spaced

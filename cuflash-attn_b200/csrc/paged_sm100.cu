@@ -357,20 +357,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr int R = G::kSlots;
     extern __shared__ uint8_t smem_raw[];
     const PagedLine& ln = p.ln;
-    // the joining kernel's blocks may wait on the SMs this one leaves
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // what the plan reads is on its way while the barriers are set up
     const int c_lo = ln.prefix_mode ? -1 : 0;
     const int run = (ln.B - c_lo + kTcThreads - 1) / kTcThreads;  // contexts per thread
     const int c_first = c_lo + static_cast<int>(threadIdx.x) * run;
-    if (c_first < ln.B) {
-        const int* at = c_first < 0 ? ln.prefix_len : ln.seq_lens + c_first;
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
-        if (!ln.prefix_mode) asm volatile("prefetch.global.L1 [%0];" ::"l"(ln.cu_seqlens + c_first));
-    }
-    int failed = 0;  // an earlier launch's failure
-    if (threadIdx.x == 0) failed = *reinterpret_cast<const volatile int*>(&g_paged_status.code);
-
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     uint8_t* sptr = smem_raw + (sbase - raw);
@@ -419,12 +408,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
-        if (!ln.prefix_mode) ln.split[blockIdx.x].last = ln.split[gridDim.x + blockIdx.x].last = -1;
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
         prefetch_tmap(&tmQ);
         prefetch_tmap(&tmQf);
         fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    stream_wait();
+    // the joining kernel's blocks may wait on the SMs this one leaves
+    stream_release();
+    int failed = 0;  // an earlier launch's failure
+    if (threadIdx.x == 0) {
+        failed = *reinterpret_cast<const volatile int*>(&g_paged_status.code);
+        if (!ln.prefix_mode) ln.split[blockIdx.x].last = ln.split[gridDim.x + blockIdx.x].last = -1;
     }
 
     // ---- the lines: contexts' lengths summed over the block, then the context
@@ -462,10 +462,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 31) scan[l * 12 + warp] = incl;
             mine[l] = incl - mine[l];
         }
-        if (__syncthreads_or(failed)) return;
-        if (warp == 1) {
-            tmem_alloc(tmem_slot, 512);
-            tmem_relinquish();
+        if (__syncthreads_or(failed)) {
+            if (warp == 1) tmem_dealloc(*tmem_slot, 512);
+            return;
         }
         long long sum[2] = {0, 0};
 #pragma unroll 1
@@ -1470,7 +1469,7 @@ __device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, co
 
 __device__ __forceinline__ bool partials_ready() {
     // the first kernel's writes are visible behind this; nothing is read if it failed
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    stream_wait();
     return *reinterpret_cast<const volatile int*>(&g_paged_status.code) == 0;
 }
 
@@ -1491,6 +1490,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int hk = ln.chunks == 1 ? hc : hc / ln.chunks;
     const int head = hk * ln.group + (hc - hk * ln.chunks) * ln.gt + hr;
     const bool valid = tok_r < ln.tpt && b < ln.B && head < (hk + 1) * ln.group;
+    stream_release();
+    // (the first kernel let this one start when the lengths were there)
     const bool has_own = valid && ln.seq_lens[b] > 0;
     const bool has_prefix = valid && *ln.prefix_len > 0;
     if (!partials_ready()) return;
@@ -1522,6 +1523,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     __shared__ JoinSmem<T> sm;
     __shared__ int ends[2][kJoinThreads + 1];  // [light, heavy]: items of the threads before
     const PagedLine& ln = p.ln;
+    stream_release();
     if (!partials_ready()) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n_rec = 2 * ln.pieces;
@@ -1635,22 +1637,6 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
 }
 
-// Launches `kern` so that its blocks may be scheduled while the kernel before
-// it on the stream still runs (they wait for it inside).
-cudaError_t launch_behind(void (*kern)(const TcParams), dim3 grid, cudaStream_t stream,
-                          const TcParams& p) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p);
-}
-
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 template <typename T, int D, int NC>
@@ -1725,20 +1711,20 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     p.O_part = reinterpret_cast<float*>(base + off_o);
 
     bind_status_word(reinterpret_cast<const void*>(&g_paged_status), stream);
-    kern<<<grid, kTcThreads, G::kSmemBytes, stream>>>(mq, mqf, mk, mv, p);
-    cudaError_t err = cudaGetLastError();
+    cudaError_t err = launch_behind(kern, dim3(grid), kTcThreads, G::kSmemBytes, stream, mq, mqf, mk, mv, p);
     if (err == cudaSuccess) {
         if (ln.prefix_mode) {
             const int tiles = (ln.B + ln.tpt - 1) / ln.tpt;
             const int last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
             const int groups = (tiles - 1) * (kTileRows / 32) + (last + 31) / 32;
-            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kJoinCols), stream, p);
+            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kJoinCols), kJoinThreads, 0,
+                                stream, p);
         } else {
             // as many blocks as are resident at once (two per SM)
-            err = launch_behind(paged_join_split_kernel<T, D>, dim3(2 * grid), stream, p);
+            err = launch_behind(paged_join_split_kernel<T, D>, dim3(2 * grid), kJoinThreads, 0, stream, p);
         }
-        if (err != cudaSuccess) cudaGetLastError();
     }
+    if (err != cudaSuccess) cudaGetLastError();
     workspace_free(ws, stream);
     return err == cudaSuccess ? FlashAttentionError::SUCCESS : FlashAttentionError::CUDA_ERROR;
 }
