@@ -1336,7 +1336,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 // The second kernel: joins partial rows by their log2-sum-exp.  A block takes 32
 // rows (one per lane, so that loads of the partials' layout are contiguous) and
-// 32 columns; its 8 warps share the partials (warp w those at w, w + 8, ...),
+// 8 or 32 columns; its 8 warps share the partials (warp w those at w, w + 8, ...),
 // and their sums are joined through shared memory in warp order, so a result
 // depends on the lengths alone.  Bound by latency: with the maxima, weights and
 // products of all partials in one warp after the other, 37 partials took 26 us,
@@ -1344,7 +1344,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinCols = 32;
+// Columns of a block: the prefix join's blocks each know their rows, and fewer
+// columns make more of them (19 sequences behind 5003 keys, 32, 16 or 8 columns:
+// 26.9, 24.4, 23.3 us a call); the ragged one's have to find them, and more
+// columns make fewer searches (one chunk of 33 tokens: 18.4, 20.1, 23.3 us).
+constexpr int kPrefixCols = 8;
+constexpr int kSplitCols = 32;
 
 // A lane's partials: n of them, tiles of `rows` rows `step` rows apart from
 // `base` on, row r of each.
@@ -1352,37 +1357,39 @@ struct Parts {
     int n, base, step, rows, r;
 };
 
-template <typename T>
+template <typename T, int C>
 struct JoinSmem {
-    float4 acc[kJoinWarps][kJoinCols / 4][32];
+    float4 acc[kJoinWarps][C / 4][32];
     float top[kJoinWarps][32];
     float tot[kJoinWarps][32];
     int row[32];
-    __align__(16) T tile[32][kJoinCols + 8];
+    __align__(16) T tile[32][C + 8];
 };
 
 // A lane's running maximum, sum and output, and two partials into it (their
 // loads in flight together; the second may be absent).
+template <int C>
 struct JoinState {
     float top, tot;
-    float4 acc[kJoinCols / 4];
+    float4 acc[C / 4];
 };
 
-__device__ __forceinline__ void join_init(JoinState& st) {
+template <int C>
+__device__ __forceinline__ void join_init(JoinState<C>& st) {
     st.top = -INFINITY;
     st.tot = 0.f;
 #pragma unroll
-    for (int q = 0; q < kJoinCols / 4; ++q) st.acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < C / 4; ++q) st.acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 struct PartRow {
     int tile_row, rows, r;
 };
 
-template <int D>
-__device__ __forceinline__ void join_two(const TcParams& p, JoinState& st, const PartRow& a, const PartRow& b,
+template <int D, int C>
+__device__ __forceinline__ void join_two(const TcParams& p, JoinState<C>& st, const PartRow& a, const PartRow& b,
                                          bool has_b, int col0) {
-    constexpr int Q = kJoinCols / 4;
+    constexpr int Q = C / 4;
     const float4* src0 = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(a.tile_row) * D) +
                          (col0 / 4) * a.rows + a.r;
     const float4* src1 = reinterpret_cast<const float4*>(p.O_part + static_cast<long long>(b.tile_row) * D) +
@@ -1417,14 +1424,14 @@ __device__ __forceinline__ PartRow part_row(const Parts& a, const Parts& b, int 
 }
 
 // Joins the partials of both lists, a lane's row going to out_row (-1: none),
-// columns [col0, col0 + 32).
-template <typename T, int D>
-__device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, const Parts& a, const Parts& b,
+// columns [col0, col0 + C).
+template <typename T, int D, int C>
+__device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T, C>& sm, const Parts& a, const Parts& b,
                                           int out_row, int col0) {
-    constexpr int Q = kJoinCols / 4;
+    constexpr int Q = C / 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = a.n + b.n;
-    JoinState st;
+    JoinState<C> st;
     join_init(st);
 #pragma unroll 1
     for (int k = warp; k < n; k += 2 * kJoinWarps)
@@ -1436,49 +1443,51 @@ __device__ __forceinline__ void join_rows(const TcParams& p, JoinSmem<T>& sm, co
     sm.tot[warp][lane] = st.tot;
     if (warp == 0) sm.row[lane] = out_row;
     __syncthreads();
-    // warp q: columns 4 q .. 4 q + 3
-    float M = -INFINITY;
+    if (warp < Q) {  // columns 4 warp .. 4 warp + 3
+        float M = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kJoinWarps; ++u) M = fmaxf(M, sm.top[u][lane]);
-    const float M0 = M == -INFINITY ? 0.f : M;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float tot = 0.f;
+        for (int u = 0; u < kJoinWarps; ++u) M = fmaxf(M, sm.top[u][lane]);
+        const float M0 = M == -INFINITY ? 0.f : M;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float tot = 0.f;
 #pragma unroll
-    for (int u = 0; u < kJoinWarps; ++u) {
-        const float w = sm100::ex2_approx(sm.top[u][lane] - M0);
-        const float4 v = sm.acc[u][warp][lane];
-        tot = fmaf(w, sm.tot[u][lane], tot);
-        o.x = fmaf(w, v.x, o.x);
-        o.y = fmaf(w, v.y, o.y);
-        o.z = fmaf(w, v.z, o.z);
-        o.w = fmaf(w, v.w, o.w);
+        for (int u = 0; u < kJoinWarps; ++u) {
+            const float w = sm100::ex2_approx(sm.top[u][lane] - M0);
+            const float4 v = sm.acc[u][warp][lane];
+            tot = fmaf(w, sm.tot[u][lane], tot);
+            o.x = fmaf(w, v.x, o.x);
+            o.y = fmaf(w, v.y, o.y);
+            o.z = fmaf(w, v.z, o.z);
+            o.w = fmaf(w, v.w, o.w);
+        }
+        const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
+        uint2 packed;
+        packed.x = DType<T>::pack2(o.x * inv, o.y * inv);
+        packed.y = DType<T>::pack2(o.z * inv, o.w * inv);
+        *reinterpret_cast<uint2*>(&sm.tile[lane][warp * 4]) = packed;
+        if (warp == 0 && col0 == 0 && out_row >= 0)
+            p.L[out_row] = tot == 0.f ? -INFINITY : (M + __log2f(tot)) * kLn2;
     }
-    const float inv = tot > 0.f ? __fdividef(1.f, tot) : 0.f;
-    uint2 packed;
-    packed.x = DType<T>::pack2(o.x * inv, o.y * inv);
-    packed.y = DType<T>::pack2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(&sm.tile[lane][warp * 4]) = packed;
-    if (warp == 0 && col0 == 0 && out_row >= 0)
-        p.L[out_row] = tot == 0.f ? -INFINITY : (M + __log2f(tot)) * kLn2;
     __syncthreads();
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
+    const int r = threadIdx.x / (C / 8), c = threadIdx.x % (C / 8) * 8;
     if (r < 32 && sm.row[r] >= 0)
         *reinterpret_cast<uint4*>(static_cast<T*>(p.O) + static_cast<long long>(sm.row[r]) * D + col0 + c) =
             *reinterpret_cast<const uint4*>(&sm.tile[r][c]);
 }
 
-__device__ __forceinline__ bool partials_ready() {
-    // the first kernel's writes are visible behind this; nothing is read if it failed
+// The first kernel's writes are visible behind this; nonzero: it failed (asked
+// for together with the records, which are only used if it did not).
+__device__ __forceinline__ int partials_wait() {
     stream_wait();
-    return *reinterpret_cast<const volatile int*>(&g_paged_status.code) == 0;
+    return *reinterpret_cast<const volatile int*>(&g_paged_status.code);
 }
 
-// Block (32 rows of the batch's row tiles, head chunk, 32 columns): the prefix's
+// Block (32 rows of the batch's row tiles, head chunk, columns): the prefix's
 // partials, then the sequence's own.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_prefix_kernel(const __grid_constant__ TcParams p) {
-    __shared__ JoinSmem<T> sm;
+    __shared__ JoinSmem<T, kPrefixCols> sm;
     const PagedLine& ln = p.ln;
     const int hc = blockIdx.y;
     const int row = blockIdx.x * 32 + (threadIdx.x & 31);  // of the head chunk
@@ -1494,20 +1503,16 @@ __global__ void __launch_bounds__(kJoinThreads)
     // (the first kernel let this one start when the lengths were there)
     const bool has_own = valid && ln.seq_lens[b] > 0;
     const bool has_prefix = valid && *ln.prefix_len > 0;
-    if (!partials_ready()) return;
-    Parts pre = {}, own = {};
-    if (has_prefix) {
-        const int u = hc * ln.prefix_pairs + (tile >> 1);
-        const Span sp = ln.span[u];
-        pre = Parts{sp.last - sp.first + 1, (u + sp.first) * (2 * kTileRows) + (tile & 1) * kTileRows,
-                    2 * kTileRows, kTileRows, r};
-    }
-    if (has_own) {
-        const int u = b * ln.heads + hc;
-        const Span sp = ln.span[ln.heads * ln.prefix_pairs + u];
-        own = Parts{sp.last - sp.first + 1, ln.own_part_row + (u + sp.first) * ln.gt, ln.gt, ln.gt, hr};
-    }
-    join_rows<T, D>(p, sm, pre, own, valid ? b * ln.hq + head : -1, blockIdx.z * kJoinCols);
+    const int u0 = hc * ln.prefix_pairs + (tile >> 1), u1 = b * ln.heads + hc;
+    const int failed = partials_wait();
+    Span sp0 = {0, -1}, sp1 = {0, -1};
+    if (has_prefix) sp0 = ln.span[u0];
+    if (has_own) sp1 = ln.span[ln.heads * ln.prefix_pairs + u1];
+    if (__syncthreads_or(failed)) return;
+    const Parts pre = {sp0.last - sp0.first + 1, (u0 + sp0.first) * (2 * kTileRows) + (tile & 1) * kTileRows,
+                       2 * kTileRows, kTileRows, r};
+    const Parts own = {sp1.last - sp1.first + 1, ln.own_part_row + (u1 + sp1.first) * ln.gt, ln.gt, ln.gt, hr};
+    join_rows<T, D>(p, sm, pre, own, valid ? b * ln.hq + head : -1, blockIdx.z * kPrefixCols);
 }
 
 // The ragged units that several pieces share, 32 rows and 32 columns at a time.
@@ -1519,12 +1524,12 @@ constexpr int kLightParts = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_split_kernel(const __grid_constant__ TcParams p) {
-    constexpr int kColGroups = D / kJoinCols;
-    __shared__ JoinSmem<T> sm;
+    constexpr int kColGroups = D / kSplitCols;
+    __shared__ JoinSmem<T, kSplitCols> sm;
     __shared__ int ends[2][kJoinThreads + 1];  // [light, heavy]: items of the threads before
     const PagedLine& ln = p.ln;
     stream_release();
-    if (!partials_ready()) return;
+    const int failed = partials_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n_rec = 2 * ln.pieces;
     const int run = (n_rec + kJoinThreads - 1) / kJoinThreads;
@@ -1541,11 +1546,11 @@ __global__ void __launch_bounds__(kJoinThreads)
         return static_cast<unsigned>((rows + 31) / 32 * kColGroups) << (n > kLightParts ? 16 : 0);
     };
     unsigned mine = 0;
-#pragma unroll 1
+#pragma unroll 2
     for (int k = 0; k < run; ++k) mine += items(threadIdx.x * run + k);
     ends[0][threadIdx.x + 1] = mine & 0xffffu;
     ends[1][threadIdx.x + 1] = mine >> 16;
-    __syncthreads();
+    if (__syncthreads_or(failed)) return;
     if (warp < 2) {  // inclusive sums, 8 threads' counts per lane
         int v[kJoinThreads / 32], sum = 0;
 #pragma unroll
@@ -1602,7 +1607,7 @@ __global__ void __launch_bounds__(kJoinThreads)
         const int base = (few ? ln.few_part_row : tile * kTileRows) + 2 * i * slot;
         return Item{Parts{valid ? 1 : 0, base + slot, 0, rows, r},
                     Parts{valid ? sp.last - i : 0, base + 2 * slot, 2 * slot, rows, r},
-                    valid ? token * ln.hq + sp.head0 + hr : -1, left % kColGroups * kJoinCols};
+                    valid ? token * ln.hq + sp.head0 + hr : -1, left % kColGroups * kSplitCols};
     };
     const int light = ends[0][kJoinThreads], heavy = ends[1][kJoinThreads];
 #pragma unroll 1
@@ -1614,8 +1619,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     for (int at = (gridDim.x - 1 - blockIdx.x) * kJoinWarps + warp; at < light; at += gridDim.x * kJoinWarps) {
         const Item it = find(at, 0);
         if (it.out_row < 0) continue;
-        constexpr int Q = kJoinCols / 4;
-        JoinState st;
+        constexpr int Q = kSplitCols / 4;
+        JoinState<kSplitCols> st;
         join_init(st);
         const int n = it.rest.n + 1;
 #pragma unroll 1
@@ -1717,7 +1722,7 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
             const int tiles = (ln.B + ln.tpt - 1) / ln.tpt;
             const int last = (ln.B - (tiles - 1) * ln.tpt) * ln.gt;  // rows of the last tile
             const int groups = (tiles - 1) * (kTileRows / 32) + (last + 31) / 32;
-            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kJoinCols), kJoinThreads, 0,
+            err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kPrefixCols), kJoinThreads, 0,
                                 stream, p);
         } else {
             // as many blocks as are resident at once (two per SM)
