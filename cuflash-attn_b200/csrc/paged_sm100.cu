@@ -688,6 +688,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         ph ^= 1;
                     }
                 };
+                // S of the next step, a row tile's
+                auto rows_s = [&](int t) {
+                    const int qslot = mode == kTwoTiles ? i & 1 : cur_q;
+                    const uint64_t a0 = pg_kdesc<D>(sb + qslot * G::kQSlotBytes);
+                    const uint64_t b0 = pg_kdesc<D>(sb + G::kOffRing + ks * G::kTileBytes);
+                    if (leader)
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        mma_f16_ss(tm + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
+                                   kk > 0 ? 1u : 0u);
+                };
+                // behind an S: what waits for it, the step's flags, the next step
+                auto s_issued = [&](int t) -> uint32_t {
+                    commit(leader, bar_s + t);
+                    uint32_t flags = kDue | (i >= 2 ? kAcc : 0) | (i + 2 >= steps ? kLast : 0);
+                    if (mode == kTwoTiles) {
+                        if (i + 2 >= steps) commit(leader, bar_qfree + (i & 1));
+                        flags |= i & 1 ? kFreeV : kWaitV;
+                    } else {
+                        if (G::kHasFew && mode == kFew)
+                            flags |= kIsFew | (cur_q ? kQSlot1 : 0) | (i + 1 == steps ? kFreeQ : 0);
+                        else if (i + 1 == steps)
+                            commit(leader, bar_qfree + cur_q);
+                        flags |= kFreeV | kWaitV;
+                    }
+                    if (flags & kFreeV) {
+                        commit(leader, empty + ks);
+                        next_slot(ks, kph);
+                    }
+                    ++i;
+                    return flags;
+                };
                 // S of the next step (stream t); its flags, 0 at the end
                 auto issue_s = [&](int t) -> uint32_t {
                     if (i == steps) {
@@ -713,46 +745,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             qs ^= 1;
                         }
                     }
-                    const bool two = mode == kTwoTiles;
-                    const int u = two ? i & 1 : 0;
-                    if (u == 0 && !k_ready && !wait(full + ks, kph)) return 0;
+                    if (!(mode == kTwoTiles && (i & 1)) && !k_ready && !wait(full + ks, kph)) return 0;
                     k_ready = false;
-                    const int qslot = two ? u : cur_q;
                     tc_fence_after();
-                    const uint64_t a0 = pg_kdesc<D>(sb + qslot * G::kQSlotBytes);
-                    const uint64_t b0 = pg_kdesc<D>(sb + G::kOffRing + ks * G::kTileBytes);
-                    uint32_t flags = kDue | (i >= 2 ? kAcc : 0) | (i + 2 >= steps ? kLast : 0);
                     if (G::kHasFew && mode == kFew) {
+                        const uint64_t a0 = pg_kdesc<D>(sb + cur_q * G::kQSlotBytes);
+                        const uint64_t b0 = pg_kdesc<D>(sb + G::kOffRing + ks * G::kTileBytes);
                         if (leader)
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
                             mma_f16_ss(tm + t * 128, b0 + pg_kdelta<D>(kk), a0 + pg_kdelta<D>(kk), idesc_kq,
                                        kk > 0 ? 1u : 0u);
-                        flags |= kIsFew | (qslot ? kQSlot1 : 0) | (i + 1 == steps ? kFreeQ : 0);
                     } else {
-                        if (leader)
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            mma_f16_ss(tm + t * 128, a0 + pg_kdelta<D>(kk), b0 + pg_kdelta<D>(kk), idesc_qk,
-                                       kk > 0 ? 1u : 0u);
+                        rows_s(t);
                     }
-                    commit(leader, bar_s + t);
-                    if (two) {
-                        if (i + 2 >= steps) commit(leader, bar_qfree + u);
-                        flags |= u ? kFreeV : kWaitV;
-                    } else {
-                        if (i + 1 == steps && mode != kFew) commit(leader, bar_qfree + cur_q);
-                        flags |= kFreeV | kWaitV;
-                    }
-                    if (flags & kFreeV) {
-                        commit(leader, empty + ks);
-                        next_slot(ks, kph);
-                    }
-                    ++i;
-                    return flags;
+                    return s_issued(t);
                 };
-                // O of stream t's step, in step order
-                auto issue_o = [&](int t, uint32_t flags) -> bool {
+                // O of stream t's step, in step order; with `next`, the stream's next S
+                // right behind it if that is in the segment and its keys have landed
+                auto issue_o = [&](int t, uint32_t flags, uint32_t* next) -> bool {
+                    bool with_s = false;
                     const uint32_t phase = (par >> t) & 1;
                     if (flags & kWaitV) {
                         if (!wait2(full + vs, vph, bar_p + t, phase)) return false;
@@ -779,14 +791,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int kk = 0; kk < 4; ++kk)
                             mma_f16_ts(o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv,
                                        kk > 0 ? 1u : acc);
-                        const bool kr = mbar_test(full + ks, kph);
+                        const bool kr = (mode == kTwoTiles && (i & 1)) || mbar_test(full + ks, kph);
                         if (!wait(bar_p2 + t, phase)) return false;
                         k_ready = __all_sync(0xffffffffu, kr);
+                        with_s = next != nullptr && k_ready && i != steps && mode != kFew;
                         tc_fence_after();
                         if (leader)
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk)
                             mma_f16_ts(o_tm, tm + t * 128 + kk * 8, v0 + pg_vdelta<D>(kk), idesc_pv, 1u);
+                    }
+                    if (with_s) {
+                        rows_s(t);
+                        *next = s_issued(t);
+                        k_ready = false;
                     }
                     if (flags & kLast) commit(leader, bar_o + t);
                     if (flags & kFreeV) {
@@ -801,13 +819,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
                 for (int t = 0;; t ^= 1) {
                     const uint32_t mine = (due >> (16 * t)) & 0xffffu;
-                    if (mine != 0 && !issue_o(t, mine)) break;
+                    uint32_t next = 0;
+                    if (mine != 0 && !issue_o(t, mine, &next)) break;
                     // The other stream's O does not wait behind an S whose keys have
                     // not landed; and a segment of few rows ends with all its
                     // products, as the next one may need the query slot that holds P^T.
                     // (Two tiles take twice the products per key: their loads are ahead.)
                     uint32_t other = (due >> (16 * (t ^ 1))) & 0xffffu;
-                    if (mode != kTwoTiles && other != 0) {
+                    if (mode != kTwoTiles && other != 0 && next == 0) {
                         bool now = G::kHasFew && mode == kFew && i == steps;
 #pragma unroll 1
                         while (!now && i != steps && !__any_sync(0xffffffffu, mbar_test(full + ks, kph))) {
@@ -815,11 +834,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             if (__any_sync(0xffffffffu, *abort_flag != 0 || tick() - since > kWaitTicks)) break;
                         }
                         if (now) {
-                            if (!issue_o(t ^ 1, other)) break;
+                            if (!issue_o(t ^ 1, other, nullptr)) break;
                             other = 0;
                         }
                     }
-                    const uint32_t next = end ? 0 : issue_s(t);
+                    if (next == 0 && !end) next = issue_s(t);
                     due = (next << (16 * t)) | (other << (16 * (t ^ 1)));
                     if (!ok || due == 0) break;
                 }
