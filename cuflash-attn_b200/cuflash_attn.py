@@ -220,14 +220,11 @@ def _mismatch(name, t, shape):
     return CuFlashError(DIMENSION_MISMATCH, f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
 
 
-def _token_stride(t, dtype, device: int, shape, name: str) -> int:
+def _token_stride(t, dtype, device: int, tokens: int, heads: int, D: int, name: str) -> int:
     """Elements between tokens of t [tokens, heads, D] whose heads are packed
-    (0 where there is only one); t like `shape`, on `device`."""
-    if t.shape != shape:
-        raise _mismatch(name, t, shape)
+    (0 where there is only one); t of `dtype`, on `device`."""
     if t.dtype is not dtype:
         raise CuFlashError(UNSUPPORTED_DTYPE, f"{name} must be {dtype}, not {t.dtype}")
-    tokens, heads, D = shape
     between, head, element = t.stride()
     if element != 1 or (heads > 1 and head != D):
         raise ValueError("a token's heads must be contiguous")
@@ -255,20 +252,25 @@ class CuFlashAttn:
             fn = self._paged_fn[key] = getattr(self.lib, f"{entry}_{_suffix(t)}")
         return fn
 
-    def _call_on(self, device: int, stream, fn, pack, *args) -> None:
-        """fn(pack(*args, stream)) with `device` current; by default on its
-        current stream."""
+    def _call_on(self, device: int, fn, args: bytes) -> None:
+        """fn(args) with `device` current."""
         import torch
 
-        raw = (torch._C._cuda_getCurrentRawStream(device) if stream is None
-               else stream.cuda_stream)
         if torch._C._cuda_getDevice() == device:
-            code = fn(pack(*args, raw))
+            code = fn(args)
         else:
             with torch.cuda.device(device):
-                code = fn(pack(*args, raw))
+                code = fn(args)
         if code:
             self.check_error(code)
+
+    @staticmethod
+    def _raw_stream(device: int, stream) -> int:
+        """The stream's handle; by default that of the device's current one."""
+        import torch
+
+        return (torch._C._cuda_getCurrentRawStream(device) if stream is None
+                else stream.cuda_stream)
 
     def error_string(self, code: int) -> str:
         return self.lib.cuflash_error_string(int(code)).decode("utf-8")
@@ -395,15 +397,15 @@ class CuFlashAttn:
         import torch
 
         tokens, Hkv, D = shape = K.shape
-        num_pages, page_size, cache_heads, cache_dim = K_cache.shape
+        num_pages, page_size, cache_heads, cache_dim = cache_shape = K_cache.shape
         B, max_pages = block_table.shape
         dtype, device = K.dtype, K.get_device()
         if V.shape != shape:
             raise _mismatch("V", V, shape)
         if cache_heads != Hkv or cache_dim != D:
             raise _mismatch("K_cache", K_cache, (num_pages, page_size, Hkv, D))
-        if V_cache.shape != K_cache.shape:
-            raise _mismatch("V_cache", V_cache, K_cache.shape)
+        if V_cache.shape != cache_shape:
+            raise _mismatch("V_cache", V_cache, cache_shape)
         if seq_lens.shape != (B,):
             raise _mismatch("seq_lens", seq_lens, (B,))
         ints = (block_table, seq_lens)
@@ -422,16 +424,18 @@ class CuFlashAttn:
                 and _packed_on(device, dtype, (K_cache, V_cache))):
             _require(device, (dtype, {"K_cache": K_cache, "V_cache": V_cache}),
                      (torch.int32, {f"index tensor {i}": t for i, t in enumerate(ints)}))
-        k_stride = _token_stride(K, dtype, device, shape, "K")
-        v_stride = _token_stride(V, dtype, device, shape, "V")
+        k_stride = _token_stride(K, dtype, device, tokens, Hkv, D, "K")
+        v_stride = _token_stride(V, dtype, device, tokens, Hkv, D, "V")
         Hq = q_stride = q_ptr = out_ptr = rope_ptr = max_position = rotary = 0
         if Q is not None:
-            Hq = Q.shape[1]
-            q_stride = _token_stride(Q, dtype, device, (tokens, Hq, D), "Q")
+            q_tokens, Hq, q_dim = q_shape = Q.shape
+            if q_tokens != tokens or q_dim != D:
+                raise _mismatch("Q", Q, (tokens, Hq, D))
+            q_stride = _token_stride(Q, dtype, device, tokens, Hq, D, "Q")
             if Q_out is None:
-                Q_out = torch.empty((tokens, Hq, D), device=Q.device, dtype=dtype)
-            elif Q_out.shape != Q.shape:
-                raise _mismatch("Q_out", Q_out, Q.shape)
+                Q_out = torch.empty(q_shape, device=Q.device, dtype=dtype)
+            elif Q_out.shape != q_shape:
+                raise _mismatch("Q_out", Q_out, q_shape)
             elif not _packed_on(device, dtype, (Q_out,)):
                 _require(device, (dtype, {"Q_out": Q_out}))
             q_ptr, out_ptr = Q.data_ptr(), Q_out.data_ptr()
@@ -442,12 +446,11 @@ class CuFlashAttn:
                 _require(device, (torch.float32, {"rope_table": rope_table}))
             max_position, rotary = rope_table.shape
             rope_ptr = rope_table.data_ptr()
-        self._call_on(device, stream, self._paged("cuflash_kv_append_paged_args", K),
-                      APPEND_ARGS.pack, q_ptr, K.data_ptr(), V.data_ptr(), out_ptr,
-                      K_cache.data_ptr(), V_cache.data_ptr(), rope_ptr, pos_ptr,
-                      block_table.data_ptr(), seq_lens.data_ptr(), cu_ptr, q_stride, k_stride,
-                      v_stride, tokens, B, Hq, Hkv, D, page_size, max_pages, num_pages, rotary,
-                      max_position, bool(interleaved))
+        self._call_on(device, self._paged("cuflash_kv_append_paged_args", K), APPEND_ARGS.pack(
+            q_ptr, K.data_ptr(), V.data_ptr(), out_ptr, K_cache.data_ptr(), V_cache.data_ptr(),
+            rope_ptr, pos_ptr, block_table.data_ptr(), seq_lens.data_ptr(), cu_ptr, q_stride,
+            k_stride, v_stride, tokens, B, Hq, Hkv, D, page_size, max_pages, num_pages, rotary,
+            max_position, bool(interleaved), self._raw_stream(device, stream)))
         return Q_out
 
     def forward_paged(self, Q, K_cache, V_cache, block_table, seq_lens, cu_seqlens,
@@ -476,11 +479,12 @@ class CuFlashAttn:
                      (torch.int32, {"block_table": block_table, "seq_lens": seq_lens,
                                     "cu_seqlens": cu_seqlens}))
         O, L = self._outputs(Q, device, shape, (tokens, Hq), O, L)
-        self._call_on(device, stream, self._paged("cuflash_attention_forward_paged_args", Q),
-                      PAGED_ARGS.pack, Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), 0, 0,
-                      block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-                      O.data_ptr(), L.data_ptr(), tokens, B, Hq, Hkv, D, page_size, 0, max_pages,
-                      num_pages, bool(causal), D ** -0.5 if scale is None else scale)
+        self._call_on(
+            device, self._paged("cuflash_attention_forward_paged_args", Q), PAGED_ARGS.pack(
+                Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), 0, 0, block_table.data_ptr(),
+                seq_lens.data_ptr(), cu_seqlens.data_ptr(), O.data_ptr(), L.data_ptr(), tokens, B,
+                Hq, Hkv, D, page_size, 0, max_pages, num_pages, bool(causal),
+                D ** -0.5 if scale is None else scale, self._raw_stream(device, stream)))
         return O, L
 
     def decode_shared_prefix(self, q, K_cache, V_cache, prefix_table, prefix_len, block_table,
@@ -516,13 +520,13 @@ class CuFlashAttn:
                      (torch.int32, {"prefix_table": prefix_table, "prefix_len": prefix_len,
                                     "block_table": block_table, "seq_lens": seq_lens}))
         O, L = self._outputs(q, device, shape, (B, Hq), O, L)
-        self._call_on(device, stream,
-                      self._paged("cuflash_attention_decode_shared_prefix_args", q),
-                      PAGED_ARGS.pack, q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(),
-                      prefix_table.data_ptr(), prefix_len.data_ptr(), block_table.data_ptr(),
-                      seq_lens.data_ptr(), 0, O.data_ptr(), L.data_ptr(), B, B, Hq, Hkv, D,
-                      page_size, max_prefix, max_pages, num_pages, False,
-                      D ** -0.5 if scale is None else scale)
+        self._call_on(
+            device, self._paged("cuflash_attention_decode_shared_prefix_args", q), PAGED_ARGS.pack(
+                q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), prefix_table.data_ptr(),
+                prefix_len.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0,
+                O.data_ptr(), L.data_ptr(), B, B, Hq, Hkv, D, page_size, max_prefix, max_pages,
+                num_pages, False, D ** -0.5 if scale is None else scale,
+                self._raw_stream(device, stream)))
         return O, L
 
     @staticmethod
