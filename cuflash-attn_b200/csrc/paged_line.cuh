@@ -46,9 +46,13 @@ constexpr int kFewTile = 16;  // rows of a partial tile of few rows (ragged)
 #define CUFLASH_ROLLED
 #endif
 
-// What a unit costs besides its keys, in keys: with 127, a unit of row tiles
-// weighs as much as its key blocks.
-constexpr int kUnitCost = 127;
+// What a unit costs besides its keys, in keys: 64 for the unused part of its last
+// block, on average, and 1.5 blocks for the start and the end of a segment (3.3 us,
+// where a block of two row tiles takes 2.3).  Too little, and the CTAs with short
+// units are late: 16 mixed sequences take 113.8, 111.4, 108.9 and 111.9 us with
+// 127, 191, 255 and 319, a prefix of 32768 keys before 128 sequences 159, 155, 154
+// and 157 with 127, 191, 255 and 383.
+constexpr int kUnitCost = 255;
 
 enum UnitMode { kOneTile = 0, kTwoTiles = 1, kFew = 2 };
 enum Line { kTiles = 0, kFewLine = 1 };
@@ -165,7 +169,9 @@ __host__ __device__ __forceinline__ int line_of(const Ctx& c) {
 }
 
 // Length of a piece: at least a block of a two-tile unit, so that every piece
-// between a unit's first and last one has a block of it.
+// between a unit's first and last one has a block of it.  (Longer ones make fewer
+// partials to join, but a step costs more than that: one chunk of 33 tokens takes
+// 18.0 us with 256, 22.9 with 384, 22.3 with 512.)
 __host__ __device__ __forceinline__ long long piece_length(long long line, int pieces) {
     const int shift = line >> 31 ? 20 : 0;
     const long long per =

@@ -1539,6 +1539,11 @@ __global__ void __launch_bounds__(kJoinThreads)
 // partials, the usual kind, are joined by single warps, a lane per row, without
 // any exchange; the others by whole blocks as above.
 constexpr int kLightParts = 4;
+struct Record {
+    int tok0, head0, parts;
+    int nh_tokens;  // heads << 16 | tokens (256 at most)
+};
+constexpr int kMaxRecords = 2 * kJoinThreads;  // two per thread; two per SM
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
@@ -1546,6 +1551,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     constexpr int kColGroups = D / kSplitCols;
     __shared__ JoinSmem<T, kSplitCols> sm;
     __shared__ int ends[2][kJoinThreads + 1];  // [light, heavy]: items of the threads before
+    __shared__ Record recs[kMaxRecords];
     const PagedLine& ln = p.ln;
     stream_release();
     const int failed = partials_wait();
@@ -1553,20 +1559,27 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int n_rec = 2 * ln.pieces;
     const int run = (n_rec + kJoinThreads - 1) / kJoinThreads;
     auto piece_of = [&](int i) -> int { return i < ln.pieces ? i : i - ln.pieces; };
-    // items of record i (light in the low half, heavy in the high half): groups of
-    // 32 rows times groups of columns
-    auto items = [&](int i) -> unsigned {
-        if (i >= n_rec) return 0;
+    // record i, and its items (light in the low half, heavy in the high half):
+    // groups of 32 rows times groups of columns
+    auto record = [&](int i) -> Record {
         const Split sp = ln.split[i];
-        const int n = sp.last - piece_of(i) + 1;
-        if (n <= 1) return 0;
-        const int tokens = min(sp.tok_end - sp.tok0, sp.mode == kTwoTiles ? 2 * ln.tpt : ln.tpt);
+        return Record{sp.tok0, sp.head0, sp.last - piece_of(i) + 1,
+                      sp.nh << 16 | min(sp.tok_end - sp.tok0, sp.mode == kTwoTiles ? 2 * ln.tpt : ln.tpt)};
+    };
+    auto items = [&](const Record& u) -> unsigned {
+        if (u.parts <= 1) return 0;
+        const int tokens = u.nh_tokens & 0xffff;
         const int rows = tokens > ln.tpt ? kTileRows + (tokens - ln.tpt) * ln.gt : tokens * ln.gt;
-        return static_cast<unsigned>((rows + 31) / 32 * kColGroups) << (n > kLightParts ? 16 : 0);
+        return static_cast<unsigned>((rows + 31) / 32 * kColGroups) << (u.parts > kLightParts ? 16 : 0);
     };
     unsigned mine = 0;
-#pragma unroll 2
-    for (int k = 0; k < run; ++k) mine += items(threadIdx.x * run + k);
+    if (threadIdx.x * run < n_rec) {  // a thread's two loads are in flight together
+        const int i0 = threadIdx.x * run, i1 = min(i0 + run - 1, n_rec - 1);
+        const Record a = record(i0), b = record(i1);
+        recs[i0] = a;
+        recs[i1] = b;
+        mine = items(a) + (i1 > i0 ? items(b) : 0);
+    }
     ends[0][threadIdx.x + 1] = mine & 0xffffu;
     ends[1][threadIdx.x + 1] = mine >> 16;
     if (__syncthreads_or(failed)) return;
@@ -1604,13 +1617,12 @@ __global__ void __launch_bounds__(kJoinThreads)
         }
         int left = at - ends[kind][owner], rec = owner * run;
         auto of_kind = [&](unsigned v) -> int { return static_cast<int>(kind ? v >> 16 : v & 0xffffu); };
-        int n = of_kind(items(rec));
-#pragma unroll 1
-        while (left >= n) {
+        const int n = of_kind(items(recs[rec]));
+        if (left >= n) {
             left -= n;
-            n = of_kind(items(++rec));
+            ++rec;
         }
-        const Split sp = ln.split[rec];
+        const Record u = recs[rec];
         const bool few = rec >= ln.pieces;
         const int i = piece_of(rec);
         const int row = left / kColGroups * 32 + lane;
@@ -1618,15 +1630,15 @@ __global__ void __launch_bounds__(kJoinThreads)
         const int r = row % kTileRows;
         const int tok_r = r / ln.gt;
         const int hr = r - tok_r * ln.gt;
-        const int token = sp.tok0 + tile * ln.tpt + tok_r;
-        const bool valid = tok_r < ln.tpt && hr < sp.nh && token < sp.tok_end;
+        const int token = tile * ln.tpt + tok_r;  // of the unit
+        const bool valid = tok_r < ln.tpt && hr < (u.nh_tokens >> 16) && token < (u.nh_tokens & 0xffff);
         // piece i's last segment, then the first ones of the pieces behind it
         const int rows = few ? kFewTile : kTileRows;      // of a tile
         const int slot = few ? kFewTile : 2 * kTileRows;  // of a segment
         const int base = (few ? ln.few_part_row : tile * kTileRows) + 2 * i * slot;
         return Item{Parts{valid ? 1 : 0, base + slot, 0, rows, r},
-                    Parts{valid ? sp.last - i : 0, base + 2 * slot, 2 * slot, rows, r},
-                    valid ? token * ln.hq + sp.head0 + hr : -1, left % kColGroups * kSplitCols};
+                    Parts{valid ? u.parts - 1 : 0, base + 2 * slot, 2 * slot, rows, r},
+                    valid ? (u.tok0 + token) * ln.hq + u.head0 + hr : -1, left % kColGroups * kSplitCols};
     };
     const int light = ends[0][kJoinThreads], heavy = ends[1][kJoinThreads];
 #pragma unroll 1
@@ -1691,7 +1703,7 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     p.few_tok = std::max(1, kFewRows / ln.gt);
     const int grid = persistent_grid(0x7fffffffLL, 1);
     long long rows, records;
-    if (!set_parts(ln, grid, rows, records) || ln.heads > 65535) return FlashAttentionError::INVALID_DIMENSION;
+    if (!set_parts(ln, grid, rows, records) || ln.heads > 65535 || 2 * grid > kMaxRecords) return FlashAttentionError::INVALID_DIMENSION;
 
     const CUtensorMapDataType dt = DType<T>::kTmaType;
     const CUtensorMapSwizzle swz = G::kSwz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
