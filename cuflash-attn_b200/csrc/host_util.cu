@@ -67,6 +67,16 @@ bool encode_tmap_3d_strided(CUtensorMap* map, const void* base, CUtensorMapDataT
     return r == CUDA_SUCCESS;
 }
 
+namespace {
+// One-time set-up may fall into a capture (the process's first call captured):
+// none of it is the captured stream's work, so it runs in the relaxed mode.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 bool ensure_smem_attr(const void* kernel, int bytes) {
     // (device, kernel, bytes) already configured; a plain table keeps the
     // library from exporting standard-container template instances.
@@ -84,6 +94,7 @@ bool ensure_smem_attr(const void* kernel, int bytes) {
     std::lock_guard<std::mutex> lock(mu);
     for (int i = 0; i < n_done; ++i)
         if (done[i].dev == dev && done[i].kernel == kernel && done[i].bytes >= bytes) return true;
+    const RelaxedCapture relaxed;
     int optin = 0;
     if (cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) !=
         cudaSuccess)
@@ -194,6 +205,7 @@ FlashAttentionError workspace_alloc(void** ptr, size_t bytes, cudaStream_t strea
     {
         std::lock_guard<std::mutex> lock(mu);
         if (pools[dev] == nullptr) {
+            const RelaxedCapture relaxed;
             cudaMemPoolProps props = {};
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;

@@ -710,6 +710,84 @@ def test_two_streams_at_once(lib, cuda):
             assert torch.equal(O, O2) and torch.equal(L, L2)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_from_another_stream(lib, cuda, captured):
+    """Calls back to back, each after a wait for a stream that writes its inputs
+    (queries, keys, lengths) late: the kernels start behind the one before them,
+    but read nothing before what they wait for is there."""
+    import torch
+
+    B, Hq, Hkv, D = 6, 8, 2, 64
+    c = Cache([400] * B, 16, Hkv, D, torch.bfloat16, 41)
+    k0 = c.K.clone()
+    rounds = 8
+    srcs = [(_randn(c.gen, B, Hq + 2 * Hkv, D, dtype=torch.bfloat16), _i32([40 * (i + 1)] * B))
+            for i in range(rounds)]
+    qkv, lens, cu = torch.zeros_like(srcs[0][0]), _i32([1] * B), _cu([1] * B)
+    burn = torch.zeros(1 << 25, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(src):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            burn.add_(1.0)
+            qkv.copy_(src[0])
+            lens.copy_(src[1])
+        main.wait_stream(side)
+        lib.kv_append_paged(qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:], c.K, c.V, c.table, lens)
+        return lib.forward_paged(qkv[:, :Hq].contiguous(), c.K, c.V, c.table, lens, cu)
+
+    want = []
+    for src in srcs:
+        want.append(step(src))
+        torch.cuda.synchronize()
+    c.K.copy_(k0)
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = [step(src) for src in srcs]
+        graph.replay()
+    else:
+        got = [step(src) for src in srcs]
+    torch.cuda.synchronize()
+    for (O, L), (O2, L2) in zip(got, want):
+        assert torch.equal(O, O2) and torch.equal(L, L2)
+
+
+def test_first_call_is_captured(cuda):
+    """In a new process, the first calls may be captured ones."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch, cuflash_attn as cf
+lib = cf.CuFlashAttn()
+t = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+K, V, q, k = t(8, 16, 2, 64), t(8, 16, 2, 64), t(2, 4, 64), t(2, 2, 64)
+table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+lens = torch.tensor([60, 17], dtype=torch.int32, device="cuda")
+cu = torch.arange(3, dtype=torch.int32, device="cuda")
+plen = torch.tensor([16], dtype=torch.int32, device="cuda")
+rope = cf.rope_table(64, 64)
+def step():
+    r = lib.kv_append_paged(k, k, K, V, table, lens, Q=q, rope_table=rope)
+    return (*lib.forward_paged(r, K, V, table, lens, cu),
+            *lib.decode_shared_prefix(r.unsqueeze(2), K, V, table[0, :1].contiguous(), plen, table, lens))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+want = step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and lib.device_status() == 0
+"""
+    root = Path(__file__).resolve().parents[1]
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root / "cuflash-attn_b200")
+
+
 @pytest.mark.parametrize("reserve", [1, 147])
 def test_reserved_sms(lib, cuda, reserve):
     """Fewer CTAs cut the work into fewer pieces."""
