@@ -1775,7 +1775,9 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
             err = launch_behind(paged_join_prefix_kernel<T, D>, dim3(groups, ln.heads, D / kPrefixCols), kJoinThreads, 0,
                                 stream, p);
         } else {
-            // as many blocks as are resident at once (two per SM)
+            // As many blocks as are resident at once, two per SM (three, with fewer
+            // registers: 16 mixed sequences 110.0 us against 112.6, but a chunk of 33
+            // tokens 18.2 against 16.9).
             err = launch_behind(paged_join_split_kernel<T, D>, dim3(2 * grid), kJoinThreads, 0, stream, p);
         }
     }
