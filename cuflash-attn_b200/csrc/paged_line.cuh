@@ -193,6 +193,21 @@ __host__ __device__ __forceinline__ int quotient(long long y, long long d) {
     return q;
 }
 
+// The piece of a line that CTA `cta` takes.
+__host__ __device__ __forceinline__ int piece_index(const PagedLine& p, int line, int cta) {
+    return line == kTiles ? cta : p.pieces - 1 - cta;
+}
+
+// Ragged: no unit starts in the CTA's pieces until its walk of them says so.  A
+// CTA resets the records that its own walk writes, and no others: nothing orders
+// it with another CTA, which may have walked its pieces before this one starts
+// (where a kernel on another stream holds the SM), so a reset of that one's
+// records would lose them, and with them the rows of the units they name.
+__host__ __device__ __forceinline__ void reset_records(const PagedLine& p, int cta) {
+    p.split[piece_index(p, kTiles, cta)].last = -1;
+    p.split[p.pieces + piece_index(p, kFewLine, cta)].last = -1;
+}
+
 // Piece [x0, x1) of a line, unit by unit.
 struct Walk {
     Ctx ctx;

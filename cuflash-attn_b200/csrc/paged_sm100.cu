@@ -442,13 +442,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int failed = 0;  // an earlier launch's failure
     if (threadIdx.x == 0) {
         failed = *reinterpret_cast<const volatile int*>(&g_paged_status.code);
-        if (!ln.prefix_mode) ln.split[blockIdx.x].last = ln.split[gridDim.x + blockIdx.x].last = -1;
+        if (!ln.prefix_mode) reset_records(ln, static_cast<int>(blockIdx.x));
     }
 
     // ---- the lines: contexts' lengths summed over the block, then the context
     // each of this CTA's pieces starts in
-    const int n_cta = static_cast<int>(gridDim.x);
-    long long mine[2] = {0, 0};  // pass 0: lengths; pass 1: position behind the contexts so far
+        long long mine[2] = {0, 0};  // pass 0: lengths; pass 1: position behind the contexts so far
     Ctx ctx = {};
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -496,11 +495,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (threadIdx.x < 2) {
             const long long line = threadIdx.x == kTiles ? sum[0] : sum[1];
-            const int piece = threadIdx.x == kTiles ? static_cast<int>(blockIdx.x)
-                                                    : n_cta - 1 - static_cast<int>(blockIdx.x);
+            const int piece = piece_index(ln, static_cast<int>(threadIdx.x), static_cast<int>(blockIdx.x));
             Start& st = start[threadIdx.x];
             st.c = -2;
-            st.per = piece_length(line, n_cta);
+            st.per = piece_length(line, ln.pieces);
             st.x0 = min(piece * st.per, line);
             st.x1 = min(st.x0 + st.per, line);
         }
@@ -920,8 +918,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (start[l].c < c_lo) continue;
                 Walk w;
                 walk_start(ln, w, start[l].ctx, start[l].c, start[l].base, start[l].x0, start[l].x1, start[l].per, l,
-                           l == kTiles ? static_cast<int>(blockIdx.x) : n_cta - 1 - static_cast<int>(blockIdx.x),
-                           lane == 0);
+                           piece_index(ln, l, static_cast<int>(blockIdx.x)), lane == 0);
 #pragma unroll 1
                 while (ok && walk_next(ln, w, sg, next_ctx)) emit(sg);
             }
