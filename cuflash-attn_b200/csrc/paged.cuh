@@ -13,6 +13,13 @@ __host__ __device__ __forceinline__ int clamp_len(int n, int most) {
     return n < 0 ? 0 : (n < most ? n : most);
 }
 
+// Keys of a sequence of `len` that a token sees, the from_end-th from its end: at
+// most len, also where offsets that do not ascend put a token behind the end (its
+// keys would lie behind the table).
+__host__ __device__ __forceinline__ int visible_keys(int len, int from_end, int causal) {
+    return causal && from_end > 1 ? len - (from_end - 1) : len;
+}
+
 #ifdef __CUDACC__
 // Launches `kern` so that its blocks may be scheduled while the kernel before
 // it on the stream still runs: every thread calls stream_wait() before it

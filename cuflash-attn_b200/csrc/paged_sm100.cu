@@ -147,9 +147,8 @@ __global__ void __launch_bounds__(kRowThreads)
     };
     if (p.prefix_table != nullptr)
         attend(p.prefix_table, clamp_len(*p.prefix_len, p.max_prefix_pages << p.page_shift));
-    int n = min(max(p.seq_lens[b], 0), p.max_pages << p.page_shift);
-    if (p.causal) n -= from_end - 1;
-    attend(p.block_table + static_cast<long long>(b) * p.max_pages, n);
+    attend(p.block_table + static_cast<long long>(b) * p.max_pages,
+           visible_keys(clamp_len(p.seq_lens[b], p.max_pages << p.page_shift), from_end, p.causal));
 
     if (li == 0) {
         s_m[grp] = m;
