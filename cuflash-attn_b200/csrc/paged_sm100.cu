@@ -1542,14 +1542,19 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int head = hk * ln.group + (hc - hk * ln.chunks) * ln.gt + hr;
     const bool valid = tok_r < ln.tpt && b < ln.B && head < (hk + 1) * ln.group;
     stream_release();
-    // (the first kernel let this one start when the lengths were there)
-    const bool has_own = valid && ln.seq_lens[b] > 0;
-    const bool has_prefix = valid && *ln.prefix_len > 0;
     const int u0 = hc * ln.prefix_pairs + (tile >> 1), u1 = b * ln.heads + hc;
     const int failed = partials_wait();
-    Span sp0 = {0, -1}, sp1 = {0, -1};
-    if (has_prefix) sp0 = ln.span[u0];
-    if (has_own) sp1 = ln.span[ln.heads * ln.prefix_pairs + u1];
+    // lengths and spans are asked for together: a unit without keys has no span, and
+    // what stands in its place is not used
+    const Span none = {0, -1};
+    Span sp0 = none, sp1 = none;
+    if (valid) {
+        const int own_len = ln.seq_lens[b], prefix_len = *ln.prefix_len;
+        sp0 = ln.span[u0];
+        sp1 = ln.span[ln.heads * ln.prefix_pairs + u1];
+        if (prefix_len <= 0) sp0 = none;
+        if (own_len <= 0) sp1 = none;
+    }
     if (__syncthreads_or(failed)) return;
     const Parts pre = {sp0.last - sp0.first + 1, (u0 + sp0.first) * (2 * kTileRows) + (tile & 1) * kTileRows,
                        2 * kTileRows, kTileRows, r};
