@@ -76,6 +76,13 @@ struct Seg {
 };
 static_assert(sizeof(Seg) == 64, "Seg layout");
 
+// How long a wait for a segment of n_blk blocks may last, in ticks of 1024 ns:
+// `base`, the limit of a wait for a single block, and 64 for each block (they take
+// 2 to 4 us).
+__host__ __device__ __forceinline__ unsigned wait_ticks(unsigned base, int n_blk) {
+    return base + 64u * static_cast<unsigned>(n_blk);
+}
+
 // The pieces of a unit: written by the one with its first block.  Prefix decode:
 // of every unit; ragged: of the units that several pieces share, by piece.
 struct Span {

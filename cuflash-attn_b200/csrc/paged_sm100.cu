@@ -509,28 +509,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = *tmem_slot;
 
     // Bounded waits, short enough to be inlined everywhere: a wait gives up when
-    // the role's segment has lasted the limit or another role has given up; the
-    // role that ran out records it on its way out.
+    // it has lasted the limit or another role has given up; the role that ran out
+    // records it on its way out.  All but one are for a block or so of another
+    // role; warp 2's is for a whole segment.  (A limit on the time since a segment's
+    // start failed at segments of some 200 million keys, and its clock, alive over
+    // the whole segment, cost spills: long chunks 1688 us a call in a graph, 1643
+    // so.)
     bool ok = true;
     auto tick = [] { return static_cast<uint32_t>(globaltimer_ns() >> 10); };  // about 1 us
     constexpr uint32_t kWaitTicks = static_cast<uint32_t>(kWaitTimeoutNs >> 10);
-    uint32_t since = tick();
     auto poll = [&](uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t addr = smem_u32(bar);
+        if (mbar_try_wait(addr, parity)) return true;
+        const uint32_t since = tick();
 #pragma unroll 1
-        while (!mbar_try_wait(addr, parity))
+        do {
             if (*abort_flag || tick() - since > kWaitTicks) return false;
+        } while (!mbar_try_wait(addr, parity));
         return true;
     };
     // The same for waits that are not urgent: a polling warp takes issue slots
     // from the softmax warps of its quarter.
-    auto poll_idle = [&](uint64_t* bar, uint32_t parity, unsigned ns) -> bool {
+    auto poll_idle = [&](uint64_t* bar, uint32_t parity, unsigned ns, uint32_t ticks) -> bool {
         const uint32_t addr = smem_u32(bar);
+        if (mbar_try_wait(addr, parity)) return true;
+        const uint32_t since = tick();
 #pragma unroll 1
-        while (!mbar_try_wait(addr, parity)) {
-            if (*abort_flag || tick() - since > kWaitTicks) return false;
+        do {
+            if (*abort_flag || tick() - since > ticks) return false;
             __nanosleep(ns);
-        }
+        } while (!mbar_try_wait(addr, parity));
         return true;
     };
 
@@ -583,7 +591,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
                 if (sg.n_blk == 0) break;
-                since = tick();
                 int chunk = sg.blk0 >> chunk_shift;
                 int entry = entry_next_seg;
                 if (!have_next) entry = load_entry(sg, chunk);
@@ -597,7 +604,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
                     for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
                         const int slot = sg.mode == kTwoTiles ? u : qs;
-                        if (q_cnt[slot] > 0) ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20);
+                        if (q_cnt[slot] > 0) ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20, kWaitTicks);
                         if (!ok) break;
                         mbar_arrive_expect_tx(bar_q + slot, bytes);
                         for (int cb = 0; cb < G::kNumCb; ++cb)
@@ -635,7 +642,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int row0 = (page << ln.page_shift) + (row & ((1 << ln.page_shift) - 1));
                     if (lane == 0) {
                         // the first lap's waits pass: no fill has used the slot
-                        if (fills + v >= R) ok = poll_idle(empty + slot_kv, phase, 20);
+                        if (fills + v >= R) ok = poll_idle(empty + slot_kv, phase, 20, kWaitTicks);
                         if (ok)
                             mbar_arrive_expect_tx(full + slot_kv,
                                                   static_cast<uint32_t>(nbox << box_shift) * G::kRowBytes);
@@ -754,7 +761,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         i = 0;
                         end = steps == 0;
                         if (end) return 0;
-                        since = tick();
                         if (mode == kTwoTiles) {
                             steps *= 2;
                             if (!wait(bar_q, qph & 1) || !wait(bar_q + 1, qph >> 1)) return 0;
@@ -851,10 +857,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint32_t other = (due >> (16 * (t ^ 1))) & 0xffffu;
                     if (mode != kTwoTiles && other != 0 && next == 0) {
                         bool now = G::kHasFew && mode == kFew && i == steps;
+                        uint32_t since = 0;  // of the second round
 #pragma unroll 1
                         while (!now && i != steps && !__any_sync(0xffffffffu, mbar_test(full + ks, kph))) {
                             now = __any_sync(0xffffffffu, mbar_test(bar_p + (t ^ 1), (par >> (t ^ 1)) & 1));
-                            if (__any_sync(0xffffffffu, *abort_flag != 0 || tick() - since > kWaitTicks)) break;
+                            if (since == 0) since = tick() | 1;
+                            if (__any_sync(0xffffffffu, *abort_flag != 0 || tick() - since > kWaitTicks + 1)) break;
                         }
                         if (now) {
                             if (!issue_o(t ^ 1, other, nullptr)) break;
@@ -878,13 +886,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // neighbours in the other one.
             unsigned smid;
             asm volatile("mov.u32 %0, %%smid;" : "=r"(smid));
-            int k = 0;
+            int k = 0, longest = 0;  // segments; blocks of the longest, which a wait may be for
             auto emit = [&](const Seg& sg) {
                 if (k >= kSegRing)
-                    ok = __all_sync(0xffffffffu,
-                                    poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500));
+                    ok = __all_sync(0xffffffffu, poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500,
+                                                           wait_ticks(kWaitTicks, longest)));
                 if (!ok) return;
-                since = tick();
+                longest = max(longest, sg.n_blk);
                 if (lane == 0) {
                     segs[k % kSegRing] = sg;
                     mbar_arrive(seg_full + k % kSegRing);
@@ -1161,7 +1169,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_free + k % kSegRing);
             if (sg.n_blk == 0) break;
-            since = tick();
             const bool two = sg.mode == kTwoTiles;
             const int first = (t ^ n0) & 1;  // two tiles: this stream's tile; else: its first block
             const int n = two ? sg.n_blk : (sg.n_blk - first + 1) / 2;
