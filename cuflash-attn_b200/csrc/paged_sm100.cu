@@ -862,7 +862,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         while (!now && i != steps && !__any_sync(0xffffffffu, mbar_test(full + ks, kph))) {
                             now = __any_sync(0xffffffffu, mbar_test(bar_p + (t ^ 1), (par >> (t ^ 1)) & 1));
                             if (since == 0) since = tick() | 1;
-                            if (__any_sync(0xffffffffu, *abort_flag != 0 || tick() - since > kWaitTicks + 1)) break;
+                            if (__any_sync(0xffffffffu, *abort_flag != 0 || static_cast<int>(tick() - since) >
+                                                                                static_cast<int>(kWaitTicks)))
+                                break;
                         }
                         if (now) {
                             if (!issue_o(t ^ 1, other, nullptr)) break;
