@@ -140,8 +140,8 @@ Option g_options[] = {
     {"CUFLASH_CP_WAVES", {-1}},          // context-parallel forward step grid
     {"CUFLASH_DECODE_GQA_TC", {-1}},     // 0 selects the SIMT grouped-query decode
     {"CUFLASH_FAULT_WORKSPACE_OOM", {-1}},  // 1 fails every workspace request (tests)
-    // tests of the bounded waits (fp16/bf16 forward only): wait limit in ms
-    // (unset: 4 s), and 1 = CTA 0 leaves out its first K load
+    // tests of the bounded waits (fp16/bf16 forward, paged attention): wait limit
+    // in ms (unset: 4 s), and 1 = CTA 0's first keys never arrive
     {"CUFLASH_TEST_WAIT_LIMIT_MS", {-1}},
     {"CUFLASH_TEST_SKIP_K_LOAD", {-1}},
 };

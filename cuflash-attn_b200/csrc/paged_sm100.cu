@@ -282,6 +282,8 @@ struct TcParams {
     int few_tok;  // tokens of the few-rows query box
     int num_pages;
     float scale_log2;
+    uint32_t wait_ticks;  // limit of a wait, in ticks of 1024 ns
+    int hold_keys;        // tests: the first CTA's first keys never count as landed
 };
 
 template <int D>
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(bar_m + t, 4);
         }
         for (int s = 0; s < R; ++s) {
-            mbar_init(full + s, 1);
+            mbar_init(full + s, s == 0 && blockIdx.x == 0 && p.hold_keys ? 2 : 1);
             mbar_init(empty + s, 1);
         }
         mbar_init(bar_x, 128);
@@ -517,14 +519,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // so.)
     bool ok = true;
     auto tick = [] { return static_cast<uint32_t>(globaltimer_ns() >> 10); };  // about 1 us
-    constexpr uint32_t kWaitTicks = static_cast<uint32_t>(kWaitTimeoutNs >> 10);
     auto poll = [&](uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t addr = smem_u32(bar);
         if (mbar_try_wait(addr, parity)) return true;
         const uint32_t since = tick();
 #pragma unroll 1
         do {
-            if (*abort_flag || tick() - since > kWaitTicks) return false;
+            if (*abort_flag || tick() - since > p.wait_ticks) return false;
         } while (!mbar_try_wait(addr, parity));
         return true;
     };
@@ -604,7 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
                     for (int u = 0; u < (sg.mode == kTwoTiles ? 2 : 1) && ok; ++u) {
                         const int slot = sg.mode == kTwoTiles ? u : qs;
-                        if (q_cnt[slot] > 0) ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20, kWaitTicks);
+                        if (q_cnt[slot] > 0) ok = poll_idle(bar_qfree + slot, (q_cnt[slot] - 1) & 1, 20, p.wait_ticks);
                         if (!ok) break;
                         mbar_arrive_expect_tx(bar_q + slot, bytes);
                         for (int cb = 0; cb < G::kNumCb; ++cb)
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int row0 = (page << ln.page_shift) + (row & ((1 << ln.page_shift) - 1));
                     if (lane == 0) {
                         // the first lap's waits pass: no fill has used the slot
-                        if (fills + v >= R) ok = poll_idle(empty + slot_kv, phase, 20, kWaitTicks);
+                        if (fills + v >= R) ok = poll_idle(empty + slot_kv, phase, 20, p.wait_ticks);
                         if (ok)
                             mbar_arrive_expect_tx(full + slot_kv,
                                                   static_cast<uint32_t>(nbox << box_shift) * G::kRowBytes);
@@ -665,11 +666,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // fills that are the newest of their slots (older ones were consumed).
             if (lane == 0) {
                 volatile int never = 0;
+                const unsigned long long ns = static_cast<unsigned long long>(p.wait_ticks) << 10;
                 for (int t = 0; t < 2; ++t)
-                    if (q_cnt[t] > 0) mbar_wait(bar_q + t, (q_cnt[t] - 1) & 1, &never, &g_paged_status);
+                    if (q_cnt[t] > 0) mbar_wait(bar_q + t, (q_cnt[t] - 1) & 1, &never, &g_paged_status, ns);
                 const int old = max(fills - R - v, 0);
                 for (int g = old + (old & 1) + v; g < fills; g += 2)
-                    mbar_wait(full + g % R, (g / R) & 1, &never, &g_paged_status);
+                    mbar_wait(full + g % R, (g / R) & 1, &never, &g_paged_status, ns);
             }
             __syncwarp();
         } else if (warp == 1) {
@@ -863,7 +865,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             now = __any_sync(0xffffffffu, mbar_test(bar_p + (t ^ 1), (par >> (t ^ 1)) & 1));
                             if (since == 0) since = tick() | 1;
                             if (__any_sync(0xffffffffu, *abort_flag != 0 || static_cast<int>(tick() - since) >
-                                                                                static_cast<int>(kWaitTicks)))
+                                                                                static_cast<int>(p.wait_ticks)))
                                 break;
                         }
                         if (now) {
@@ -892,7 +894,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto emit = [&](const Seg& sg) {
                 if (k >= kSegRing)
                     ok = __all_sync(0xffffffffu, poll_idle(seg_free + k % kSegRing, (k / kSegRing - 1) & 1, 500,
-                                                           wait_ticks(kWaitTicks, longest)));
+                                                           wait_ticks(p.wait_ticks, longest)));
                 if (!ok) return;
                 longest = max(longest, sg.n_blk);
                 if (lane == 0) {
@@ -1716,6 +1718,10 @@ FlashAttentionError paged_tc(const PagedParams<T>& a, cudaStream_t stream) {
     p.num_pages = a.num_pages;
     // a zero scale becomes a tiny positive one so that masked scores stay -inf
     p.scale_log2 = fmaxf(a.scale_log2, 1e-30f);
+    const int limit_ms = std::min(env_int("CUFLASH_TEST_WAIT_LIMIT_MS", 0), 100000);
+    const unsigned long long limit_ns = limit_ms > 0 ? limit_ms * 1000000ull : sm100::kWaitTimeoutNs;
+    p.wait_ticks = static_cast<uint32_t>(limit_ns >> 10);
+    p.hold_keys = env_int("CUFLASH_TEST_SKIP_K_LOAD", 0) != 0;
     ln.prefix_len = a.prefix_len;
     ln.seq_lens = a.seq_lens;
     ln.cu_seqlens = a.cu_seqlens;

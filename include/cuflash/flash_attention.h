@@ -527,10 +527,11 @@ CUFLASH_EXPORT int cuflash_profile_read_ms(float* ms, int max_launches);
 //   CUFLASH_FAULT_WORKSPACE_OOM  1 makes every workspace request fail with
 //                                OUT_OF_MEMORY (host-side fault injection);
 //   CUFLASH_TEST_WAIT_LIMIT_MS   bounded-wait limit of the fp16/bf16 forward
-//                                in ms (default 4000);
-//   CUFLASH_TEST_SKIP_K_LOAD     1 makes the fp16/bf16 forward's first CTA
-//                                leave out one K load, so that one of its
-//                                waits runs out (tests of the timeout path).
+//                                and of the tensor-core attention over a
+//                                paged cache, in ms (default 4000);
+//   CUFLASH_TEST_SKIP_K_LOAD     1 lets the first keys of these kernels' first
+//                                CTA never arrive, so that its waits for them
+//                                run out (tests of the timeout path).
 // Returns SUCCESS, NULL_POINTER, or INVALID_DIMENSION for an unknown name.
 CUFLASH_EXPORT int cuflash_set_option(const char* name, int value);
 
