@@ -20,7 +20,7 @@
 // look-ups (sequence, length, page) overlap them.  The partner of an element
 // is half a rotation away in the same head and is fetched from the owning lane
 // by a shuffle.  Measured, at those sizes: 26915 tokens in 103 us (6.5 TB/s of
-// elements, the rate of a plain copy); 256 tokens every 3.1 us inside a graph,
+// elements, the rate of a plain copy); 256 tokens every 3.0 us inside a graph,
 // which is the launch and the chain of look-ups.
 
 #include "common.cuh"

@@ -6,12 +6,12 @@
 // (ragged), or the shared prefix with every sequence's token, and each
 // sequence's own keys with its one token (prefix decode).  The query heads of
 // one K/V head (in chunks of gt <= 128 of them) are packed with the tokens
-// into row tiles of tpt tokens x gt heads <= 128 rows, so that every key and
-// value is read once for all of them.  A unit is one head chunk with two row
-// tiles, with one where no second is left, or with few rows (at most few_rows
-// in the whole context).  Its length is the number of keys its last token
-// sees plus kUnitCost, doubled for two tiles; key block j (128 keys) lies at
-// 128 j of it.  The units, one after the other (context, then head chunk, then
+// into row tiles of tpt tokens x gt heads <= 128 rows.  A unit is one head chunk
+// with two row tiles, with one where no second is left, or with few rows (at most
+// few_rows in the whole context); it reads its keys and values once for all of its
+// rows, up to 256, so a context's are read once per unit of a head chunk.  Its
+// length is the number of keys its last token sees plus kUnitCost, doubled for two
+// tiles; key block j (128 keys) lies at 128 j of it.  The units, one after the other (context, then head chunk, then
 // row tiles), form a line that is cut into equal pieces, one per CTA.  There
 // are two lines: units of row tiles, which the tensor cores bound, and units
 // of few rows, which the loads of keys and values bound; CTA i takes piece i
@@ -48,10 +48,10 @@ constexpr int kFewTile = 16;  // rows of a partial tile of few rows (ragged)
 
 // What a unit costs besides its keys, in keys: 64 for the unused part of its last
 // block, on average, and 1.5 blocks for the start and the end of a segment (3.3 us,
-// where a block of two row tiles takes 2.3).  Too little, and the CTAs with short
-// units are late: 16 mixed sequences take 113.8, 111.4, 108.9 and 111.9 us with
-// 127, 191, 255 and 319, a prefix of 32768 keys before 128 sequences 159, 155, 154
-// and 157 with 127, 191, 255 and 383.
+// where a block of two row tiles takes 2.2).  Too little, and the CTAs with short
+// units are late.  With 127, 191, 255 and 383, per call in a graph: 16 mixed sequences
+// 116.2, 114.6, 110.7 and 110.3 us, a prefix of 32768 keys before 128 sequences 154.4,
+// 152.2, 150.7 and 154.9, one of 512 before 4 15.1, 14.7, 13.0 and 13.3.
 constexpr int kUnitCost = 255;
 
 enum UnitMode { kOneTile = 0, kTwoTiles = 1, kFew = 2 };
@@ -178,7 +178,8 @@ __host__ __device__ __forceinline__ int line_of(const Ctx& c) {
 // Length of a piece: at least a block of a two-tile unit, so that every piece
 // between a unit's first and last one has a block of it.  (Longer ones make fewer
 // partials to join, but a step costs more than that: one chunk of 33 tokens takes
-// 18.0 us with 256, 22.9 with 384, 22.3 with 512.)
+// 17.7 us with 256, 21.6 with 384, 4 sequences behind 512 keys 12.8 and 14.7, and 16
+// mixed sequences 111 either way.)
 __host__ __device__ __forceinline__ long long piece_length(long long line, int pieces) {
     const int shift = line >> 31 ? 20 : 0;
     const long long per =

@@ -211,10 +211,14 @@ FlashAttentionError paged_row(const PagedParams<T>& p, cudaStream_t stream) {
 // Bounds.  Row tiles: a block of two tiles takes 4 x 128 x 128 x D multiply-adds on
 // the tensor pipe and 2 x 128 x 128 exponentials (1024 cycles each tile on the MUFU
 // pipe), but neither is full: what a step costs is its chain (S, maximum,
-// exponentials, P, O, the next S) shared by two streams.  Measured: 1.14 us a tile
-// and block at D = 128 (1087 TFLOP/s over 12288 keys, 0.67 of cuBLAS' burst rate),
-// 1.0 us at D = 64, 0.97 at D = 32.  Few rows: the bytes of keys and values;
-// 128 sequences of 4096 keys (8 K/V heads of 128, group 4) take 327 us, 6.6 TB/s.
+// exponentials, P, O, the next S) shared by two streams.  Measured, from 256 tokens
+// of 148 heads over 6144 and 12288 keys: 1.11 us a tile and block at D = 128 (1119
+// TFLOP/s, 0.69 of cuBLAS' burst rate), 0.90 at D = 64, 0.79 at D = 32; pages of 128
+// rows, 1.08 at D = 128.  The dense forward at the same sizes: 1.02, 0.83, 0.80.
+// Few rows: the bytes of keys and values; 128 sequences of 4096 keys (8 K/V heads of
+// 128, group 4) take 320 us, 6.7 TB/s.
+// Times here and below, unless they say otherwise, are per call in a CUDA graph of 8
+// to 12 calls, which keeps short runs at the burst clock and leaves the host out.
 //
 // Partials (normalised fp32 rows with their log2-sum-exp) are kept as
 // [D/4][rows][4], so that a warp of row-per-lane threads stores and loads 512
@@ -575,9 +579,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const long long row = (static_cast<long long>(chunk) * 32 + lane) << box_shift;
                 return row < sg.len ? table[row >> ln.page_shift] : 0;
             };
-            // Units of few rows read a key and its value once for all of its head's
-            // rows, the row tiles of a prompt or prefix read theirs again (32
-            // sequences behind 4096 keys: 29.6 us without priorities, 28.3 with).
+            // Units of few rows read a key and its value once for all of the
+            // sequence's rows, the row tiles of a prompt or prefix read theirs again,
+            // so the former leave L2 first: 32 sequences behind 4096 keys 30.1 us
+            // without priorities, 28.7 with, single tokens of 128 sequences of 512 keys
+            // 59 and 56.  Tables may name a page in several rows, and then few rows do
+            // read it again; that costs less than it gains elsewhere (single tokens of
+            // 32 sequences over the same 4096 keys 75.2 us without, 76.9 with, of 128
+            // over the same 8192 keys 481 and 496), and only a look at all tables
+            // could tell the two apart.
             uint64_t once, again;
             asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
             asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
@@ -1398,9 +1408,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 // Columns of a block: the prefix join's blocks each know their rows, and fewer
-// columns make more of them (19 sequences behind 5003 keys, 32, 16 or 8 columns:
-// 26.9, 24.4, 23.3 us a call); the ragged one's have to find them, and more
-// columns make fewer searches (one chunk of 33 tokens: 18.4, 20.1, 23.3 us).
+// columns make more of them (32, 16 or 8 columns: 19 sequences behind 5003 keys 25.6,
+// 23.7, 23.3 us, 4 behind 512 14.2, 13.5, 13.0, and the largest alike, 128 behind
+// 32768 152.1, 150.4, 150.8); the ragged one's have to find them, and more columns
+// make fewer searches (32 or 16: one chunk of 33 tokens 16.9, 21.2, 16 mixed sequences
+// 110.7, 116.3).
 constexpr int kPrefixCols = 8;
 constexpr int kSplitCols = 32;
 
@@ -1578,7 +1590,8 @@ __global__ void __launch_bounds__(kJoinThreads)
 // joined by single warps, a lane per row, without any exchange; the others by
 // whole blocks as above.  Little code: in a small call most of it is fetched cold
 // (an exact count of every unit's items, 20 us instead of 17 for a chunk of 33
-// tokens).
+// tokens).  With 2, 4 or 8 partials as few: the chunk of 33 tokens 17.7, 17.7, 23.7 us,
+// 16 mixed sequences 109.2, 111.1, 114.3, 7 scored without a mask 35.5, 34.8, 34.9.
 constexpr int kLightParts = 4;
 struct Record {
     int tok0, head0, parts;
@@ -1649,7 +1662,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     // item `at` of a kind, for this lane's row.  Every record has the items of 256
     // rows; where the unit has fewer, no lane has one.  A record's are turned by
     // its number, so that a warp does not meet the same rows of one on every lap
-    // (16 mixed sequences: 115.6 us unturned).
+    // (16 mixed sequences 110.0 us, 113.1 unturned).
     auto find = [&](int at, int kind) -> Item {
         const int nth = at / kItems, rec = list[kind][nth], left = (at + 5 * nth) % kItems;
         const Record u = recs[rec];

@@ -282,16 +282,22 @@ CUFLASH_EXPORT int cuflash_kv_append_paged_f16(
 // of the n new ones sees key j iff j <= i + seq_lens[b] - n.  A token that sees
 // no key gets O = 0 and L = -inf; rows from cu_seqlens[B] on are left as they
 // were.  Sequences may have any number of new tokens, none included, so one
-// call serves prompts, chunks of prompts and single tokens together.
+// call serves prompts, chunks of prompts and single tokens together.  (New
+// tokens behind a prefix that several sequences share: their tables repeat
+// the prefix' pages, so the prefix has to end with a page.)
 //
 // For both attention entries: Q, the cache and O are 16-byte aligned (else
 // CUDA_ERROR).  Cache rows behind a sequence's length may hold anything, NaN
 // included.  Keys that causality hides from a row have weight zero in it, so
 // their value rows must be finite (0 * NaN).  Results are reproducible bit by
-// bit: how the work is divided depends on the lengths and the device, and
-// nothing is summed by atomics.  Pages of 8 rows and more run on the tensor
-// cores; smaller ones take a kernel that reads the keys once per query head
-// and token.  INVALID_DIMENSION also where num_tokens * num_q_heads or the
+// bit: how the work is divided depends on the lengths, the device and
+// CUFLASH_RESERVE_SMS, and nothing is summed by atomics.  Pages of 8 rows and
+// more run on the tensor cores, with the probabilities rounded to the input
+// type for the value product (as in the dense forward; maxima, sums and the
+// product's accumulation are fp32): the error of O is 1.3 to 1.4 times that of
+// one rounding of the exact result.  Smaller pages take a kernel that keeps
+// the probabilities in fp32 and reads the keys once per query head and token,
+// so the last bits of a result depend on the page size.  INVALID_DIMENSION also where num_tokens * num_q_heads or the
 // partial results of a call would pass 2^31 rows.
 CUFLASH_EXPORT int cuflash_attention_forward_paged_bf16(
     const __nv_bfloat16* Q, const __nv_bfloat16* K_cache, const __nv_bfloat16* V_cache,
@@ -307,8 +313,10 @@ CUFLASH_EXPORT int cuflash_attention_forward_paged_f16(
 // Decode behind a shared prefix: one query token per sequence (Q, O
 // [B, num_q_heads, 1, D], L fp32 [B, num_q_heads]) against the prefix_len[0]
 // keys of the pages prefix_table [max_prefix_pages], which every sequence of
-// the batch shares and which are read once for all of them, followed by the
-// sequence's own seq_lens[b] keys (0 or more) of block_table[b].  The result is
+// the batch shares, followed by the sequence's own seq_lens[b] keys (0 or more)
+// of block_table[b].  A K/V head's prefix is read once for every 256 of its
+// query rows (two tiles of up to 128: a group of 4 packs 64 sequences into
+// them), on pages of fewer than 8 rows once for each.  The result is
 // that of attention over both together; neither any prefix nor own key: O = 0
 // and L = -inf.
 CUFLASH_EXPORT int cuflash_attention_decode_shared_prefix_bf16(
